@@ -44,7 +44,7 @@ extern "C" {
 #define LFM_ATTN_E_DEVICE     -4 /* HIP runtime error (see lfm_attn_last_error)    */
 #define LFM_ATTN_E_NOMEM      -5 /* device allocation failed                       */
 #define LFM_ATTN_E_IO         -6 /* a file could not be written                     */
-#define LFM_ATTN_E_SCRATCH    -7 /* more split partials than the no-alloc scratch holds */
+#define LFM_ATTN_E_SCRATCH    -7 /* the scratch memory is smaller than the call needs    */
 
 typedef void *lfm_attn_stream_t; /* hipStream_t */
 
@@ -218,6 +218,23 @@ int lfm_hip_qkv_prologue(float *q, const float *k, const float *v, uint16_t *con
  * as the per-4-head slices.  x 4-byte aligned; y 4-byte aligned. */
 int lfm_hip_quantize_q8_K(const float *x, void *y_q8_K, uint32_t n_rows, uint32_t n_cols,
                           lfm_attn_stream_t stream);
+
+/* Residual addition, RMS norm and Q8_K quantization in one pass, in front of
+ * the quantized projections of a layer.  No counterpart in the reference, whose
+ * stacks run the three as separate CPU loops.  Per row of n_cols values:
+ *   h = x + residual (h = x where residual is NULL), stored in residual_out
+ *       (NULL: not stored; may be x or residual: in place),
+ *   y = h / sqrt(mean(h^2) + eps) * norm_w (NULL: no weight), stored in y as
+ *       floats (NULL: not stored),
+ *   y_q8_K = the Q8_K blocks that lfm_hip_quantize_q8_K makes of y (NULL: not
+ *       stored).
+ * The mean and y are formed in 64 bits and rounded once.  y and y_q8_K share
+ * no memory with the other arrays.  n_cols % 256 == 0 (else
+ * LFM_ATTN_E_UNSUPPORTED), at most 2^24; n_rows < 2^31; n_rows == 0 does
+ * nothing.  Float arrays 16-byte aligned, y_q8_K 4-byte. */
+int lfm_hip_add_rmsnorm_q8_K(const float *x, const float *residual, const float *norm_w, float eps,
+                             float *residual_out, float *y, void *y_q8_K, uint32_t n_rows, uint32_t n_cols,
+                             lfm_attn_stream_t stream);
 
 /* Weight types of the projections (GGML ids; blocks as in
  * tools/lfm2_cpuid_quants.c:55-127, include/lfm2_simd_avx2.h:120-158), the
@@ -429,6 +446,101 @@ int lfm_hip_lfm3_prefill_f16(const float *q, const uint16_t *k, const uint16_t *
                              int gate_is_logit, float *out, uint32_t n_seq, uint32_t n_tok, uint32_t pos_0,
                              uint32_t kv_pos0, uint64_t kv_seq_stride, uint32_t window_len, uint32_t n_head_q,
                              uint32_t n_head_kv, uint32_t head_dim, float scale, lfm_attn_stream_t stream);
+
+/* ---- paged 4-bit K/V cache ------------------------------------------------------
+ * No counterpart in the reference, whose caches are linear fp16.  One buffer of
+ * n_pages pages per attention layer; a page holds page_size consecutive
+ * positions of one sequence (a power of two from 32 to 65536), keys (normed and
+ * rotated) and values of every KV head as 4-bit codes with an fp16 scale per
+ * position and 32 dims: 4.5 bits a value, 0.28 of fp16.  A code c in 0..15 under
+ * scale d stands for d * (c - 8).
+ *
+ * Layout: page p at pages + p * (lfm_attn_paged_q4_page_bytes), in it
+ * [KV head][block of 32 positions][36 * head_dim bytes]; a block holds
+ *   K codes, 16 * head_dim bytes: the 4-byte word of position t (0..31), dim
+ *     group g (dims 32 g ..) and part r (dims 32 g + 8 r .. + 7) is at
+ *     head_dim 64:   16 * (16 r + t % 16) + 8 * (t / 16) + 4 g
+ *     head_dim 128:  1024 * (t / 16) + 16 * (16 r + t % 16) + 4 g
+ *   V codes, 16 * head_dim bytes: the word of key group j (positions 4 j ..
+ *     4 j + 3 and 16 + 4 j .. 16 + 4 j + 3) and dim x is at
+ *     1024 * (x / 64) + 16 * (16 j + x % 16) + 4 * (x / 16 % 4)
+ *   K scales, 2 * head_dim bytes, then V scales: fp16 [group][key group][8]
+ * where element e = 0..7 of a word is its nibble e / 2 + 4 * (e % 2), counted
+ * from the low end, and the 8 positions of a key group are ordered as above.
+ *
+ * Arguments all paged entry points share:
+ *   pages        the layer's buffer, 16-byte aligned
+ *   n_pages      its pages: table entries outside 0 .. n_pages - 1 mean "no page"
+ *   block_table  DEVICE int32_t [n_seq][table_stride]: entry i of a sequence is the
+ *                page of positions i * page_size ..
+ *   pos_0        DEVICE uint32_t[n_seq]: position of a sequence's first row
+ *   n_rows_seq   DEVICE uint32_t[n_seq] or NULL: a sequence's rows in this call
+ *                (at most n_rows count; NULL: n_rows each; 0: a padding sequence)
+ *   n_rows       rows per sequence in the row arrays
+ * Rows behind a sequence's last, and rows at positions that the table
+ * (table_stride * page_size positions, at most 2^31) does not reach, are left as
+ * they were in every output.  Positions without a page are not stored, not
+ * attended, and read back as zeros.  head_dim 64 or 128, page_size as above, else
+ * LFM_ATTN_E_UNSUPPORTED.  Row arrays, tables of cosines and norm weights
+ * 16-byte aligned. */
+/* Bytes of one page. */
+int lfm_attn_paged_q4_page_bytes(uint32_t page_size, uint32_t n_head_kv, uint32_t head_dim, size_t *bytes);
+
+/* Norm, rotation and storing of new rows: per row and head, RMS norm (weight
+ * [head_dim] or NULL: no norm) and NeoX rotation of q and k as in
+ * lfm_hip_qkv_prologue, but in 64 bits and rounded once; q goes to q_out (may
+ * be q: in place; q and q_out both NULL: keys and values only), k and v to the
+ * cache.  Per 32 dims of a row, with m the value of largest magnitude (the
+ * positive one of two): d = fp16(-m / 8), c = clamp(floor(x / d + 8.5), 0, 15)
+ * (all 8 where d is 0, which is kept as +0).  Groups with values that are not finite or pass fp16's
+ * range in d read back as NaN.
+ * q, q_out: [n_seq][n_rows][n_head_q][head_dim]; k, v:
+ * [n_seq][n_rows][n_head_kv][head_dim].  cos_lut / sin_lut:
+ * [lut_rows][head_dim / 2]; rows at positions >= lut_rows count as rows behind
+ * the last.  Two sequences of a call must not store into the same block of 32
+ * positions of a page (shared pages are for prefixes that are only read). */
+int lfm_hip_paged_q4_append(const float *q, const float *k, const float *v, float *q_out, void *pages,
+                            uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                            uint32_t table_stride, const uint32_t *pos_0, const uint32_t *n_rows_seq,
+                            uint32_t n_seq, uint32_t n_rows, uint32_t n_head_q, uint32_t n_head_kv,
+                            uint32_t head_dim, const float *q_norm_w, const float *k_norm_w, float eps,
+                            const float *cos_lut, const float *sin_lut, uint32_t lut_rows,
+                            lfm_attn_stream_t stream);
+
+/* Positions pos_0 .. as linear RNE fp16 rows k_out, v_out
+ * [n_seq][n_rows][n_head_kv][head_dim]: the rows that the linear-cache entry
+ * points, lfm_attn_ctx_kv_import and the cache files take. */
+int lfm_hip_paged_q4_gather(uint16_t *k_out, uint16_t *v_out, const void *pages, uint32_t n_pages,
+                            uint32_t page_size, const int32_t *block_table, uint32_t table_stride,
+                            const uint32_t *pos_0, const uint32_t *n_rows_seq, uint32_t n_seq, uint32_t n_rows,
+                            uint32_t n_head_kv, uint32_t head_dim, lfm_attn_stream_t stream);
+
+/* Attention of rows at positions pos_0 .. over the cache, which holds them
+ * already: decode (n_rows 1), verify (a few rows) and prompts (any number; the
+ * sequences may differ).  Row r of sequence s attends [t_start(p), p], p =
+ * pos_0[s] + r, t_start(p) = p + 1 - window_len where window_len > 0 and
+ * p + 1 > window_len, else 0.  gate as in lfm_hip_gqa_f16_varlen.  A row that
+ * finds no page at all gives zeros.  Outputs have fp32 accuracy with respect to
+ * the cached values.
+ * q, out: [n_seq][n_rows][n_head_q][head_dim], n_head_q a multiple of n_head_kv;
+ * q rotated.
+ * keys_hint: an upper bound of pos_0[s] + rows over the batch (0 = what the
+ * table reaches); it sizes the key split.  Longer sequences are still handled
+ * correctly, with longer shares.
+ * workspace: device scratch of the caller, 16-byte aligned, of at least
+ * lfm_attn_paged_q4_workspace_bytes for these arguments (else
+ * LFM_ATTN_E_SCRATCH, nothing launched).  It needs no initial value and holds
+ * nothing between calls; calls that may overlap need one each.  The call
+ * allocates nothing and may be captured. */
+int lfm_attn_paged_q4_workspace_bytes(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q,
+                                      uint32_t n_head_kv, uint32_t head_dim, uint32_t page_size,
+                                      uint32_t table_stride, uint32_t window_len, size_t *bytes);
+int lfm_hip_paged_q4_gqa(const float *q, const float *gate, int gate_is_logit, const void *pages, uint32_t n_pages,
+                         uint32_t page_size, const int32_t *block_table, uint32_t table_stride,
+                         const uint32_t *pos_0, const uint32_t *n_rows_seq, float *out, uint32_t n_seq,
+                         uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
+                         uint32_t head_dim, uint32_t window_len, float scale, void *workspace,
+                         size_t workspace_bytes, lfm_attn_stream_t stream);
 
 /* ---- attention-sink eviction on device caches ------------------------------ */
 /* When the position nears max_seq the engine keeps the first n_sink rows,

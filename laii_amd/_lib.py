@@ -73,6 +73,15 @@ SIGNATURES = {
                                     _u32, _u32, _u32, _u32, _f32, _vp, _vp, _f32, _vp, _vp, _int, _vp]),
     "lfm_hip_gqa_f16_varlen_noalloc": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32,
                                               _u32, _u32, _u32, _u32, _f32, _vp]),
+    "lfm_hip_add_rmsnorm_q8_K": (_int, [_vp, _vp, _vp, _f32, _vp, _vp, _vp, _u32, _u32, _vp]),
+    "lfm_attn_paged_q4_page_bytes": (_int, [_u32, _u32, _u32, C.POINTER(_sz)]),
+    "lfm_hip_paged_q4_append": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32,
+                                       _u32, _u32, _vp, _vp, _f32, _vp, _vp, _u32, _vp]),
+    "lfm_hip_paged_q4_gather": (_int, [_vp, _vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _vp]),
+    "lfm_attn_paged_q4_workspace_bytes": (_int, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
+                                                 C.POINTER(_sz)]),
+    "lfm_hip_paged_q4_gqa": (_int, [_vp, _vp, _int, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _u32, _u32,
+                                    _u32, _u32, _u32, _u32, _f32, _vp, _sz, _vp]),
     "lfm_hip_kv_cache_shift_sinks": (_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32,
                                             C.POINTER(_u32), _u32, _u32, _vp]),
     "lfm_hip_lfm3_kv_cache_shift_sinks": (_int, [_vp, _vp, _u32, _vp, _vp, _u32, _vp, _vp, _u32,

@@ -160,6 +160,15 @@ def quantize_q8_K(x: Ptr, y_q8_K: Ptr, n_rows: int, n_cols: int, stream=None) ->
           "lfm_hip_quantize_q8_K")
 
 
+def add_rmsnorm_q8_K(x: Ptr, residual: Ptr, norm_w: Ptr, eps: float, residual_out: Ptr, y: Ptr, y_q8_K: Ptr,
+                     n_rows: int, n_cols: int, stream=None) -> None:
+    """h = x + residual (stored in residual_out), y = RMS norm of h times norm_w
+    (stored in y as floats, in y_q8_K as Q8_K blocks); None for what is absent
+    or not wanted (lfm_hip_add_rmsnorm_q8_K)."""
+    check(load().lfm_hip_add_rmsnorm_q8_K(_p(x), _p(residual), _p(norm_w), eps, _p(residual_out), _p(y), _p(y_q8_K),
+                                          n_rows, n_cols, stream), "lfm_hip_add_rmsnorm_q8_K")
+
+
 def matmul_q4_K(out: Ptr, w_q4_K: Ptr, n_rows: int, n_cols: int, x_q8_K: Ptr, n_tokens: int,
                 stream=None) -> None:
     """out[t][r] = Q4_K row r . Q8_K token t (lfm2_matmul_1x4_prequant_mt,
@@ -246,6 +255,58 @@ def gqa_f16_varlen(q: Ptr, gate: Ptr, gate_is_logit: bool, k_seq: Ptr, v_seq: Pt
                                         _p(v_seq), _p(pos_0), _p(out), n_seq, n_rows,
                                         keys_hint, n_head_q, n_head_kv, head_dim, window_len,
                                         cap, scale, stream), "lfm_hip_gqa_f16_varlen")
+
+
+def paged_q4_page_bytes(page_size: int, n_head_kv: int, head_dim: int) -> int:
+    """Bytes of a page of the 4-bit cache (lfm_attn_paged_q4_page_bytes)."""
+    n = C.c_size_t(0)
+    check(load().lfm_attn_paged_q4_page_bytes(page_size, n_head_kv, head_dim, C.byref(n)),
+          "lfm_attn_paged_q4_page_bytes")
+    return int(n.value)
+
+
+def paged_q4_append(q: Ptr, k: Ptr, v: Ptr, q_out: Ptr, pages: Ptr, n_pages: int, page_size: int, block_table: Ptr,
+                    table_stride: int, pos_0: Ptr, n_rows_seq: Ptr, n_seq: int, n_rows: int, n_head_q: int,
+                    n_head_kv: int, head_dim: int, q_norm_w: Ptr, k_norm_w: Ptr, eps: float, cos_lut: Ptr,
+                    sin_lut: Ptr, lut_rows: int, stream=None) -> None:
+    """Norm and rotation of new rows, q to q_out, k and v as 4-bit blocks to
+    their pages (lfm_hip_paged_q4_append)."""
+    check(load().lfm_hip_paged_q4_append(_p(q), _p(k), _p(v), _p(q_out), _p(pages), n_pages, page_size,
+                                         _p(block_table), table_stride, _p(pos_0), _p(n_rows_seq), n_seq, n_rows,
+                                         n_head_q, n_head_kv, head_dim, _p(q_norm_w), _p(k_norm_w), eps, _p(cos_lut),
+                                         _p(sin_lut), lut_rows, stream), "lfm_hip_paged_q4_append")
+
+
+def paged_q4_gather(k_out: Ptr, v_out: Ptr, pages: Ptr, n_pages: int, page_size: int, block_table: Ptr,
+                    table_stride: int, pos_0: Ptr, n_rows_seq: Ptr, n_seq: int, n_rows: int, n_head_kv: int,
+                    head_dim: int, stream=None) -> None:
+    """Positions of a paged 4-bit cache as linear fp16 rows (lfm_hip_paged_q4_gather)."""
+    check(load().lfm_hip_paged_q4_gather(_p(k_out), _p(v_out), _p(pages), n_pages, page_size, _p(block_table),
+                                         table_stride, _p(pos_0), _p(n_rows_seq), n_seq, n_rows, n_head_kv, head_dim,
+                                         stream), "lfm_hip_paged_q4_gather")
+
+
+def paged_q4_workspace_bytes(n_seq: int, n_rows: int, keys_hint: int, n_head_q: int, n_head_kv: int, head_dim: int,
+                             page_size: int, table_stride: int, window_len: int = 0) -> int:
+    """Scratch bytes that paged_q4_gqa needs for these arguments."""
+    n = C.c_size_t(0)
+    check(load().lfm_attn_paged_q4_workspace_bytes(n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, page_size,
+                                                   table_stride, window_len, C.byref(n)),
+          "lfm_attn_paged_q4_workspace_bytes")
+    return int(n.value)
+
+
+def paged_q4_gqa(q: Ptr, gate: Ptr, gate_is_logit: bool, pages: Ptr, n_pages: int, page_size: int, block_table: Ptr,
+                 table_stride: int, pos_0: Ptr, n_rows_seq: Ptr, out: Ptr, n_seq: int, n_rows: int, keys_hint: int,
+                 n_head_q: int, n_head_kv: int, head_dim: int, workspace: Ptr, workspace_bytes: int,
+                 window_len: int = 0, scale: Optional[float] = None, stream=None) -> None:
+    """Attention over a paged 4-bit cache (lfm_hip_paged_q4_gqa)."""
+    if scale is None:
+        scale = float(1.0 / np.sqrt(np.float32(head_dim)))
+    check(load().lfm_hip_paged_q4_gqa(_p(q), _p(gate), int(bool(gate_is_logit)), _p(pages), n_pages, page_size,
+                                      _p(block_table), table_stride, _p(pos_0), _p(n_rows_seq), _p(out), n_seq,
+                                      n_rows, keys_hint, n_head_q, n_head_kv, head_dim, window_len, scale,
+                                      _p(workspace), workspace_bytes, stream), "lfm_hip_paged_q4_gqa")
 
 
 def rope_row_gen1(head_dim: int, pos: int, theta: float):

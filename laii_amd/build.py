@@ -23,7 +23,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["shim.hip", "decode_splitkv.hip", "generic.hip", "prologue.hip", "prefill_fa.hip",
-               "prefill_ext.hip", "kv_shift.hip", "quant_matmul.hip", "fnv_hash.hip", "peak_probe.hip"]
+               "prefill_ext.hip", "kv_shift.hip", "quant_matmul.hip", "fnv_hash.hip", "peak_probe.hip",
+               "norm_quant.hip", "paged_q4.hip", "paged_q4_attn.hip"]
 C_SOURCES = ["lfm_attn_host.c", "lfm_attn_ctx.c"]
 
 HIP_FLAGS = [
@@ -45,7 +46,7 @@ HIP_FLAGS = [
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 HIP_FILE_FLAGS = {"prefill_fa.hip": ["-fno-honor-nans"], "prefill_ext.hip": ["-fno-honor-nans"],
                   "decode_splitkv.hip": VGPR_MFMA, "quant_matmul.hip": VGPR_MFMA,
-                  "peak_probe.hip": VGPR_MFMA}
+                  "peak_probe.hip": VGPR_MFMA, "paged_q4_attn.hip": VGPR_MFMA}
 C_FLAGS = ["-std=c11", "-O2", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__",
            f"-I{ROCM}/include", f"-I{CSRC}", f"-I{INCLUDE}"]
 

@@ -139,6 +139,37 @@ int launch_quantize_q8_K(const float *x, void *y, uint32_t n_rows, uint32_t n_co
 int launch_matmul_q(uint32_t n_mats, float *const *outs, const void *const *ws, const uint32_t *types,
                     const uint32_t *rows, uint32_t n_cols, const void *x_q8, uint32_t n_tokens, hipStream_t stream);
 
+/* Residual addition + RMS norm + Q8_K (norm_quant.hip); n_cols % 256 == 0. */
+int launch_add_rmsnorm_q8_K(const float *x, const float *residual, const float *norm_w, float eps,
+                            float *residual_out, float *y, void *y_q8, uint32_t n_rows, uint32_t n_cols,
+                            hipStream_t stream);
+
+/* Paged 4-bit K/V cache (layout: paged_q4.h) and the rows of one call:
+ * sequence s has rows_seq[s] (or n_rows) rows from position pos0[s]; page
+ * table[s * table_stride + i] holds its positions from i * page size. */
+struct PagedQ4 {
+    uint8_t *pages;
+    const int32_t *table;
+    const uint32_t *pos0, *rows_seq; /* device; rows_seq may be null */
+    uint64_t page_bytes;
+    uint32_t n_pages, table_stride;
+    uint32_t blk_shift; /* log2 of the blocks of 32 positions per page */
+    uint32_t capacity;  /* positions a table row reaches, <= 2^31 */
+    uint32_t n_seq, n_rows, n_head_kv, head_dim;
+};
+/* Whether the append's grid has fewer than 2^31 workgroups. */
+bool paged_q4_append_fits(const PagedQ4 &c, uint32_t n_head_q);
+int launch_paged_q4_append(const PagedQ4 &c, const float *q, const float *k, const float *v, float *q_out,
+                           uint32_t n_head_q, const float *q_norm_w, const float *k_norm_w, float eps,
+                           const float *cos_lut, const float *sin_lut, uint32_t lut_rows, hipStream_t stream);
+int launch_paged_q4_gather(const PagedQ4 &c, uint16_t *k_out, uint16_t *v_out, hipStream_t stream);
+/* Scratch bytes of the attention; LFM_ATTN_E_UNSUPPORTED for a grid past 2^31. */
+int paged_q4_gqa_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
+                           uint32_t head_dim, uint32_t capacity, uint32_t window, size_t *bytes);
+int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int gate_is_logit, float *out,
+                        uint32_t n_head_q, uint32_t keys_hint, uint32_t window, float scale, void *workspace,
+                        hipStream_t stream);
+
 /* Attention-sink eviction (kv_shift.hip).  launch_kv_shift moves rows
  * [n_sink + n_discard, n_sink + n_discard + n_keep) down to n_sink and
  * counter-rotates the keys; launch_kv_swa_repack re-slots an SWA ring

@@ -1,0 +1,136 @@
+/*
+ * norm_quant.hip -- residual addition, RMS norm and Q8_K quantization in one
+ * pass: what stands between one layer's output and the next one's quantized
+ * projections.
+ *
+ *   h = x + residual           (fp32, written back as the new residual stream)
+ *   y = h / sqrt(mean(h^2) + eps) * w
+ *   blocks = Q8_K(y)           (as lfm_hip_quantize_q8_K quantizes y)
+ *
+ * The squares are summed and y is formed in 64 bits and rounded once to
+ * fp32: the 8-bit codes then do not depend on the order of the sum.  A row is
+ * one workgroup; each of its waves keeps its 256-value blocks in registers
+ * between the sum and the quantization, so x and residual are read once.
+ */
+#include <hip/hip_runtime.h>
+
+#include "kernels.h"
+#include "lfm_attn.h"
+#include "q8k_block.h"
+
+namespace lfm {
+namespace {
+
+constexpr uint32_t kWaves = 4u;
+
+struct NormParams {
+    const float *x, *res, *w;
+    float *res_out, *y;
+    uint8_t *q;
+    double eps;
+    uint32_t nb; /* 256-value blocks per row */
+};
+
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+
+/* h of 4 values, at float4 index i of the batch */
+__device__ __forceinline__ float4 load_h(const NormParams &p, size_t i) {
+    const float4 a = reinterpret_cast<const float4 *>(p.x)[i];
+    return p.res ? add4(a, reinterpret_cast<const float4 *>(p.res)[i]) : a;
+}
+
+__device__ __forceinline__ double sum_sq(double s, float4 h) {
+    s = fma((double)h.x, (double)h.x, s);
+    s = fma((double)h.y, (double)h.y, s);
+    s = fma((double)h.z, (double)h.z, s);
+    return fma((double)h.w, (double)h.w, s);
+}
+
+__device__ __forceinline__ void finish_block(const NormParams &p, float4 h, double r, size_t row, uint32_t b,
+                                             uint32_t lane) {
+    const size_t i = (row * p.nb + b) * 64u + lane;
+    float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    if (p.w) w = reinterpret_cast<const float4 *>(p.w)[b * 64u + lane];
+    const float v[4] = {(float)((double)h.x * r * (double)w.x), (float)((double)h.y * r * (double)w.y),
+                        (float)((double)h.z * r * (double)w.z), (float)((double)h.w * r * (double)w.w)};
+    if (p.y) reinterpret_cast<float4 *>(p.y)[i] = make_float4(v[0], v[1], v[2], v[3]);
+    if (p.q) quant_q8k_block(v, p.q + (row * p.nb + b) * kQ8K, lane);
+}
+
+/* BPW: blocks a wave keeps (rows of up to 4 * BPW blocks); 0: any row length,
+ * h re-formed from the inputs (or read back where it was written). */
+template <int BPW> __global__ __launch_bounds__(256) void k_add_rmsnorm_q8K(const NormParams p) {
+    __shared__ double part[kWaves];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const size_t row  = blockIdx.x;
+    const size_t base = row * p.nb * 64u + lane;
+    float4 h[BPW ? BPW : 1];
+    double s = 0.0;
+    if constexpr (BPW > 0) {
+#pragma unroll
+        for (int k = 0; k < BPW; ++k) {
+            const uint32_t b = wave + kWaves * (uint32_t)k;
+            if (b < p.nb) {
+                h[k] = load_h(p, base + b * 64u);
+                if (p.res_out) reinterpret_cast<float4 *>(p.res_out)[base + b * 64u] = h[k];
+                s = sum_sq(s, h[k]);
+            }
+        }
+    } else {
+        for (uint32_t b = wave; b < p.nb; b += kWaves) {
+            h[0] = load_h(p, base + b * 64u);
+            if (p.res_out) reinterpret_cast<float4 *>(p.res_out)[base + b * 64u] = h[0];
+            s = sum_sq(s, h[0]);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0u) part[wave] = s;
+    __syncthreads();
+    s = (part[0] + part[1]) + (part[2] + part[3]);
+    const double r = 1.0 / sqrt(s / (double)((uint64_t)p.nb * 256u) + p.eps);
+    if constexpr (BPW > 0) {
+#pragma unroll
+        for (int k = 0; k < BPW; ++k) {
+            const uint32_t b = wave + kWaves * (uint32_t)k;
+            if (b < p.nb) finish_block(p, h[k], r, row, b, lane);
+        }
+    } else {
+        for (uint32_t b = wave; b < p.nb; b += kWaves) {
+            const size_t i = base + b * 64u;
+            finish_block(p, p.res_out ? reinterpret_cast<const float4 *>(p.res_out)[i] : load_h(p, i), r, row, b, lane);
+        }
+    }
+}
+
+} // namespace
+
+int launch_add_rmsnorm_q8_K(const float *x, const float *residual, const float *norm_w, float eps,
+                            float *residual_out, float *y, void *y_q8, uint32_t n_rows, uint32_t n_cols,
+                            hipStream_t stream) {
+    NormParams p;
+    p.x       = x;
+    p.res     = residual;
+    p.w       = norm_w;
+    p.res_out = residual_out;
+    p.y       = y;
+    p.q       = static_cast<uint8_t *>(y_q8);
+    p.eps     = (double)eps;
+    p.nb      = n_cols / 256u;
+    const dim3 g(n_rows), t(64u * kWaves);
+    if (p.nb <= 1u * kWaves)
+        hipLaunchKernelGGL(k_add_rmsnorm_q8K<1>, g, t, 0, stream, p);
+    else if (p.nb <= 2u * kWaves)
+        hipLaunchKernelGGL(k_add_rmsnorm_q8K<2>, g, t, 0, stream, p);
+    else if (p.nb <= 4u * kWaves)
+        hipLaunchKernelGGL(k_add_rmsnorm_q8K<4>, g, t, 0, stream, p);
+    else if (p.nb <= 8u * kWaves)
+        hipLaunchKernelGGL(k_add_rmsnorm_q8K<8>, g, t, 0, stream, p);
+    else
+        hipLaunchKernelGGL(k_add_rmsnorm_q8K<0>, g, t, 0, stream, p);
+    return hip_status(hipGetLastError());
+}
+
+} // namespace lfm

@@ -47,11 +47,11 @@
 
 #include "kernels.h"
 #include "lfm_attn.h"
+#include "q8k_block.h"
 
 namespace lfm {
 namespace {
 
-constexpr uint32_t kQ8K = 292u;
 constexpr uint32_t kCus = 256u; /* compute units of an MI355X: sizes of a round of workgroups */
 
 __device__ __forceinline__ uint32_t ld32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
@@ -65,32 +65,7 @@ __global__ __launch_bounds__(256) void k_quant_q8K(const float *__restrict__ x, 
     const uint32_t t = blk / nb, b = blk - t * nb;
     const float *xb = x + ((size_t)t * nb + b) * 256u + 4u * lane;
     const float v[4] = {xb[0], xb[1], xb[2], xb[3]};
-    float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    uint8_t *out = y + (size_t)blk * kQ8K;
-    if (amax == 0.0f) {
-        *reinterpret_cast<uint32_t *>(out + 4u + 4u * lane) = 0u;
-        if (lane < 16u) *reinterpret_cast<int16_t *>(out + 260u + 2u * lane) = 0;
-        if (lane == 0u) *reinterpret_cast<float *>(out) = 0.0f;
-        return;
-    }
-    const float d      = amax / 127.0f;  /* correctly rounded (HIP default) */
-    const float iscale = 127.0f / amax;
-    int32_t q[4], part = 0;
-    uint32_t packed = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        q[i] = (int32_t)__builtin_rintf(v[i] * iscale); /* one rounding, then half-even */
-        part += q[i];
-        const int32_t s = q[i] > 127 ? 127 : (q[i] < -128 ? -128 : q[i]);
-        packed |= (uint32_t)(uint8_t)(int8_t)s << (8 * i);
-    }
-    *reinterpret_cast<uint32_t *>(out + 4u + 4u * lane) = packed;
-    part += __shfl_xor(part, 1);
-    part += __shfl_xor(part, 2);
-    if ((lane & 3u) == 0u) *reinterpret_cast<int16_t *>(out + 260u + (lane >> 1)) = (int16_t)part;
-    if (lane == 0u) *reinterpret_cast<float *>(out) = d;
+    quant_q8k_block(v, y + (size_t)blk * kQ8K, lane);
 }
 
 /* 6-bit scale and min of sub-block j (get_scale_min_k4,

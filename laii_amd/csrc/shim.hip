@@ -13,6 +13,7 @@
 #include "attn_index.h"
 #include "kernels.h"
 #include "lfm_attn.h"
+#include "paged_q4.h"
 
 namespace lfm {
 
@@ -138,7 +139,7 @@ const char *lfm_attn_status_string(int status) {
     case LFM_ATTN_E_DEVICE: return "device error";
     case LFM_ATTN_E_NOMEM: return "out of device memory";
     case LFM_ATTN_E_IO: return "file could not be written";
-    case LFM_ATTN_E_SCRATCH: return "split partials exceed the no-alloc scratch";
+    case LFM_ATTN_E_SCRATCH: return "split partials exceed the scratch memory";
     default: return "unknown status";
     }
 }
@@ -363,6 +364,19 @@ int lfm_hip_quantize_q8_K(const float *x, void *y_q8_K, uint32_t n_rows, uint32_
     if (n_cols % 256u) return LFM_ATTN_E_UNSUPPORTED;
     if (!aligned(x, 4) || !aligned(y_q8_K, 4)) return LFM_ATTN_E_INVALID;
     return lfm::launch_quantize_q8_K(x, y_q8_K, n_rows, n_cols, to_stream(stream));
+}
+
+int lfm_hip_add_rmsnorm_q8_K(const float *x, const float *residual, const float *norm_w, float eps,
+                             float *residual_out, float *y, void *y_q8_K, uint32_t n_rows, uint32_t n_cols,
+                             lfm_attn_stream_t stream) {
+    if (n_rows == 0u) return LFM_ATTN_OK;
+    if (!x || (!residual_out && !y && !y_q8_K) || n_cols == 0u || n_rows >= 0x80000000u) return LFM_ATTN_E_INVALID;
+    if (n_cols % 256u || n_cols > (1u << 24)) return LFM_ATTN_E_UNSUPPORTED;
+    if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(norm_w, 16) || !aligned(residual_out, 16) ||
+        !aligned(y, 16) || !aligned(y_q8_K, 4))
+        return LFM_ATTN_E_INVALID;
+    return lfm::launch_add_rmsnorm_q8_K(x, residual, norm_w, eps, residual_out, y, y_q8_K, n_rows, n_cols,
+                                        to_stream(stream));
 }
 
 int lfm_hip_matmul_q4_K(float *out, const void *w_q4_K, uint32_t n_rows, uint32_t n_cols,
@@ -676,6 +690,123 @@ int lfm_hip_lfm3_prefill_f16(const float *q, const uint16_t *k, const uint16_t *
     return lfm::launch_prefill_ext(q, k, v, gate, gate_is_logit, out, n_seq, n_tok, pos_0, kv_pos0,
                                    kv_seq_stride, window_len, n_head_q, n_head_kv, head_dim, scale,
                                    to_stream(stream));
+}
+
+/* ---- paged 4-bit K/V cache ---------------------------------------------------- */
+static int paged_shape(uint32_t page_size, uint32_t n_head_kv, uint32_t head_dim, size_t *page_bytes) {
+    if (n_head_kv == 0u) return LFM_ATTN_E_INVALID;
+    if ((head_dim != 64u && head_dim != 128u) || page_size < LFM_Q4_BLOCK || page_size > 65536u ||
+        (page_size & (page_size - 1u)) != 0u || n_head_kv > 4096u)
+        return LFM_ATTN_E_UNSUPPORTED;
+    *page_bytes = (size_t)n_head_kv * (page_size / LFM_Q4_BLOCK) * lfm_q4_block_bytes(head_dim);
+    return LFM_ATTN_OK;
+}
+
+static int paged_cache(lfm::PagedQ4 *c, const void *pages, uint32_t n_pages, uint32_t page_size,
+                       const int32_t *block_table, uint32_t table_stride, const uint32_t *pos_0,
+                       const uint32_t *n_rows_seq, uint32_t n_seq, uint32_t n_rows, uint32_t n_head_kv,
+                       uint32_t head_dim) {
+    if (!pages || !block_table || !pos_0 || n_pages == 0u || table_stride == 0u || n_seq == 0u || n_rows == 0u)
+        return LFM_ATTN_E_INVALID;
+    size_t page_bytes = 0;
+    const int st      = paged_shape(page_size, n_head_kv, head_dim, &page_bytes);
+    if (st != LFM_ATTN_OK) return st;
+    if (!aligned(pages, 16) || !aligned(block_table, 4) || !aligned(pos_0, 4) || !aligned(n_rows_seq, 4))
+        return LFM_ATTN_E_INVALID;
+    const uint64_t reach = (uint64_t)table_stride * page_size;
+    if (reach > 0x80000000ull || n_pages > 0x7FFFFFFFu) return LFM_ATTN_E_UNSUPPORTED;
+    c->pages        = static_cast<uint8_t *>(const_cast<void *>(pages));
+    c->table        = block_table;
+    c->pos0         = pos_0;
+    c->rows_seq     = n_rows_seq;
+    c->page_bytes   = page_bytes;
+    c->n_pages      = n_pages;
+    c->table_stride = table_stride;
+    c->blk_shift    = (uint32_t)__builtin_ctz(page_size / LFM_Q4_BLOCK);
+    c->capacity     = (uint32_t)reach;
+    c->n_seq        = n_seq;
+    c->n_rows       = n_rows;
+    c->n_head_kv    = n_head_kv;
+    c->head_dim     = head_dim;
+    return LFM_ATTN_OK;
+}
+
+int lfm_attn_paged_q4_page_bytes(uint32_t page_size, uint32_t n_head_kv, uint32_t head_dim, size_t *bytes) {
+    if (!bytes) return LFM_ATTN_E_INVALID;
+    return paged_shape(page_size, n_head_kv, head_dim, bytes);
+}
+
+int lfm_hip_paged_q4_append(const float *q, const float *k, const float *v, float *q_out, void *pages,
+                            uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                            uint32_t table_stride, const uint32_t *pos_0, const uint32_t *n_rows_seq,
+                            uint32_t n_seq, uint32_t n_rows, uint32_t n_head_q, uint32_t n_head_kv,
+                            uint32_t head_dim, const float *q_norm_w, const float *k_norm_w, float eps,
+                            const float *cos_lut, const float *sin_lut, uint32_t lut_rows,
+                            lfm_attn_stream_t stream) {
+    lfm::PagedQ4 c;
+    const int st = paged_cache(&c, pages, n_pages, page_size, block_table, table_stride, pos_0, n_rows_seq, n_seq,
+                               n_rows, n_head_kv, head_dim);
+    if (st != LFM_ATTN_OK) return st;
+    if (!k || !v || (q == nullptr) != (q_out == nullptr) || (q && n_head_q == 0u) || !cos_lut || !sin_lut ||
+        lut_rows == 0u)
+        return LFM_ATTN_E_INVALID;
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16) || !aligned(q_norm_w, 16) ||
+        !aligned(k_norm_w, 16) || !aligned(cos_lut, 16) || !aligned(sin_lut, 16))
+        return LFM_ATTN_E_INVALID;
+    if (!lfm::paged_q4_append_fits(c, q ? n_head_q : 0u)) return LFM_ATTN_E_UNSUPPORTED;
+    return lfm::launch_paged_q4_append(c, q, k, v, q_out, n_head_q, q_norm_w, k_norm_w, eps, cos_lut, sin_lut,
+                                       lut_rows, to_stream(stream));
+}
+
+int lfm_hip_paged_q4_gather(uint16_t *k_out, uint16_t *v_out, const void *pages, uint32_t n_pages,
+                            uint32_t page_size, const int32_t *block_table, uint32_t table_stride,
+                            const uint32_t *pos_0, const uint32_t *n_rows_seq, uint32_t n_seq, uint32_t n_rows,
+                            uint32_t n_head_kv, uint32_t head_dim, lfm_attn_stream_t stream) {
+    lfm::PagedQ4 c;
+    const int st = paged_cache(&c, pages, n_pages, page_size, block_table, table_stride, pos_0, n_rows_seq, n_seq,
+                               n_rows, n_head_kv, head_dim);
+    if (st != LFM_ATTN_OK) return st;
+    if (!k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)) return LFM_ATTN_E_INVALID;
+    if (!lfm::paged_q4_append_fits(c, 0u)) return LFM_ATTN_E_UNSUPPORTED;
+    return lfm::launch_paged_q4_gather(c, k_out, v_out, to_stream(stream));
+}
+
+int lfm_attn_paged_q4_workspace_bytes(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q,
+                                      uint32_t n_head_kv, uint32_t head_dim, uint32_t page_size,
+                                      uint32_t table_stride, uint32_t window_len, size_t *bytes) {
+    if (!bytes || n_seq == 0u || n_rows == 0u || n_head_q == 0u || n_head_kv == 0u || n_head_q % n_head_kv != 0u ||
+        table_stride == 0u)
+        return LFM_ATTN_E_INVALID;
+    size_t page_bytes = 0;
+    const int st      = paged_shape(page_size, n_head_kv, head_dim, &page_bytes);
+    if (st != LFM_ATTN_OK) return st;
+    const uint64_t reach = (uint64_t)table_stride * page_size;
+    if (reach > 0x80000000ull) return LFM_ATTN_E_UNSUPPORTED;
+    return lfm::paged_q4_gqa_workspace(n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, (uint32_t)reach,
+                                       window_len, bytes);
+}
+
+int lfm_hip_paged_q4_gqa(const float *q, const float *gate, int gate_is_logit, const void *pages, uint32_t n_pages,
+                         uint32_t page_size, const int32_t *block_table, uint32_t table_stride,
+                         const uint32_t *pos_0, const uint32_t *n_rows_seq, float *out, uint32_t n_seq,
+                         uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
+                         uint32_t head_dim, uint32_t window_len, float scale, void *workspace,
+                         size_t workspace_bytes, lfm_attn_stream_t stream) {
+    lfm::PagedQ4 c;
+    int st = paged_cache(&c, pages, n_pages, page_size, block_table, table_stride, pos_0, n_rows_seq, n_seq, n_rows,
+                         n_head_kv, head_dim);
+    if (st != LFM_ATTN_OK) return st;
+    if (!q || !out || n_head_q == 0u || n_head_q % n_head_kv != 0u || !aligned(q, 16) || !aligned(out, 16) ||
+        !aligned(gate, 4) || !aligned(workspace, 16))
+        return LFM_ATTN_E_INVALID;
+    size_t need = 0;
+    st = lfm::paged_q4_gqa_workspace(n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, c.capacity, window_len,
+                                     &need);
+    if (st != LFM_ATTN_OK) return st;
+    if (need && !workspace) return LFM_ATTN_E_INVALID;
+    if (workspace_bytes < need) return LFM_ATTN_E_SCRATCH;
+    return lfm::launch_paged_q4_gqa(c, q, gate, gate_is_logit, out, n_head_q, keys_hint, window_len, scale, workspace,
+                                    to_stream(stream));
 }
 
 /* ---- attention-sink eviction ------------------------------------------- */
