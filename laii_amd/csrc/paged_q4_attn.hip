@@ -43,6 +43,11 @@ struct GqaParams {
     float *out;
     int gate_is_logit;
     float scale;
+    /* split: steps before each entry (sequence, tile) and in all [n_entries + 1],
+     * partial outputs [slot][cols][HD], their (m, l) [slot][cols] */
+    uint32_t *pre;
+    float *part_o;
+    float2 *part_ml;
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
@@ -75,60 +80,119 @@ __device__ __forceinline__ uint32_t pk_rtz(float a, float b) {
 __device__ __forceinline__ float half_lo(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[0]; }
 __device__ __forceinline__ float half_hi(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[1]; }
 
-template <int HD> struct Block { /* one lane's share of a block of 32 positions */
-    uint4 k[HD / 64], v[HD / 64], ks[HD / 32], vs[HD / 32];
-};
-
-template <int HD> __device__ __forceinline__ void load_block(Block<HD> &b, const uint8_t *base, uint32_t lane) {
-    const uint32_t kg = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < HD / 64; ++i) {
-        b.k[i] = *reinterpret_cast<const uint4 *>(base + i * 1024 + lane * 16u);
-        b.v[i] = *reinterpret_cast<const uint4 *>(base + 16 * HD + i * 1024 + lane * 16u);
-    }
-#pragma unroll
-    for (int g = 0; g < HD / 32; ++g) {
-        b.ks[g] = *reinterpret_cast<const uint4 *>(base + 32 * HD + g * 64 + kg * 16u);
-        b.vs[g] = *reinterpret_cast<const uint4 *>(base + 34 * HD + g * 64 + kg * 16u);
-    }
-}
-
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-/* One wave: columns of one tile over all its keys. */
-template <int HD> __global__ __launch_bounds__(256) void k_paged_gqa(const GqaParams p) {
-    constexpr int G = HD / 32, DT = HD / 16;
-    const PagedQ4 &c     = p.c;
-    const uint32_t lane  = threadIdx.x & 63u, col = lane & 15u, kg = lane >> 4;
-    const uint32_t unit  = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
-    const uint32_t h     = unit % c.n_head_kv, sc = unit / c.n_head_kv;
-    const uint32_t s     = sc / p.plan.n_ct, ct = sc - s * p.plan.n_ct;
-    if (s >= c.n_seq) return;
-    const uint32_t pos0 = uniform(c.pos0[s]);
-    const uint32_t rows = lfm_q4_rows(pos0, c.rows_seq ? uniform(c.rows_seq[s]) : c.n_rows, c.n_rows, c.capacity);
-    const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
-    if (t.n_steps == 0u) return;
+/* What one wave computes with.  HD: head_dim.  NT: tiles of 16 query columns.
+ * R: with at most 16 / R columns (NT 1), each is held R times, and copy u of it
+ * takes every R-th 16-key tile of a step: softmax work shrinks by R.  The query
+ * operand is kept R times, zero outside copy r's columns, so that the S product of
+ * tile t with copy t % R leaves each column the tile that it takes, with no
+ * selection.  NB: blocks of 32 keys per step. */
+template <int HD_, int NT_, int R_, int NB_> struct Form {
+    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_;
+    static constexpr int G = HD / 32, DT = HD / 16, TILES = 2 * NB, J = TILES / R;
+    static constexpr int COLS = R > 1 ? 16 / R : 16 * NT, STEP = 32 * NB;
+    static_assert(R == 1 || (NT == 1 && J == 1), "a copy takes one tile per step");
+};
 
-    /* this lane's column */
-    const uint32_t mul = p.plan.kv_mul, n_q = c.n_head_kv * mul;
-    const uint32_t ci = ct * p.plan.cols + col, row = ci / mul;
-    const bool live   = ci < rows * mul;
-    const size_t head = ((size_t)s * c.n_rows + row) * n_q + h * mul + (ci - row * mul);
-    const uint32_t lo = live ? lfm_q4_row_lo(pos0 + row, p.plan.window) : 0u, hi = live ? pos0 + row + 1u : 0u;
+template <class F> struct Step { /* one lane's share of a step's codes and scales */
+    uint4 k[F::NB][F::HD / 64], v[F::NB][F::HD / 64];
+    uint4 ks[F::J > 1 ? F::NB : 1][F::G], vs[F::J > 1 ? F::NB : 1][F::G]; /* J 1: .x and .y alone */
+};
 
-    half8v qh[G], ql[G];
-    float cs;
-    {
-        float x[G][8];
-        float big = 0.0f;
+/* Wave-uniform place of a step: its blocks, and whether they have pages. */
+template <class F> struct Place {
+    const uint8_t *base[F::NB];
+    bool there[F::NB];
+};
+
+template <class F>
+__device__ __forceinline__ Place<F> place_of(const PagedQ4 &c, const int32_t *table, uint32_t h, uint32_t step) {
+    Place<F> p;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+    for (int b = 0; b < F::NB; ++b) {
+        /* a step's last block may lie behind the table: its keys are masked, read the one before */
+        uint32_t blk = step * F::NB + b;
+        if (F::NB > 1 && blk * 32u >= c.capacity) blk = c.capacity / 32u - 1u;
+        const int32_t id  = table[blk >> c.blk_shift];
+        const uint32_t in = blk & ((1u << c.blk_shift) - 1u);
+        p.there[b]        = (uint32_t)id < c.n_pages;
+        p.base[b]         = c.pages + (uint64_t)(p.there[b] ? (uint32_t)id : 0u) * c.page_bytes +
+                    (uint64_t)((h << c.blk_shift) + in) * lfm_q4_block_bytes(F::HD);
+    }
+    return p;
+}
+
+template <class F> __device__ __forceinline__ void load_step(Step<F> &d, const Place<F> &p, uint32_t lane) {
+    constexpr int HD = F::HD;
+    const uint32_t kg = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < F::NB; ++b)
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i) {
+            d.k[b][i] = *reinterpret_cast<const uint4 *>(p.base[b] + i * 1024 + lane * 16u);
+            d.v[b][i] = *reinterpret_cast<const uint4 *>(p.base[b] + 16 * HD + i * 1024 + lane * 16u);
+        }
+    if constexpr (F::J > 1) {
+#pragma unroll
+        for (int b = 0; b < F::NB; ++b)
+#pragma unroll
+            for (int g = 0; g < F::G; ++g) {
+                d.ks[b][g] = *reinterpret_cast<const uint4 *>(p.base[b] + 32 * HD + g * 64 + kg * 16u);
+                d.vs[b][g] = *reinterpret_cast<const uint4 *>(p.base[b] + 34 * HD + g * 64 + kg * 16u);
+            }
+    } else { /* the 4 keys of this lane's tile */
+        const uint32_t u    = (lane & 15u) / (16u / F::R);
+        const uint8_t *base = F::NB > 1 && (u >> 1) ? p.base[F::NB - 1] : p.base[0];
+        base += 32 * HD + kg * 16u + (u & 1u) * 8u;
+#pragma unroll
+        for (int g = 0; g < F::G; ++g) {
+            const uint2 a = *reinterpret_cast<const uint2 *>(base + g * 64);
+            const uint2 z = *reinterpret_cast<const uint2 *>(base + 2 * HD + g * 64);
+            d.ks[0][g]    = make_uint4(a.x, a.y, 0u, 0u);
+            d.vs[0][g]    = make_uint4(z.x, z.y, 0u, 0u);
+        }
+    }
+}
+
+/* Queries and running state of a unit's columns. */
+template <class F> struct State {
+    half8v qh[F::NT][F::R][F::G], ql[F::NT][F::R][F::G];
+    float4v o[F::NT][F::DT];
+    float cs[F::NT], top[F::NT], m[F::NT], l[F::NT];
+    uint32_t vmax[F::NT];            /* magnitude (fp16 bits) of the V scales that m covers */
+    uint32_t lo[F::NT], hi[F::NT];   /* keys [lo, hi) of the column's row */
+};
+
+/* Index of the column's (row, head) in q, out and gate; ~0: none. */
+template <class F>
+__device__ __forceinline__ size_t head_of(const GqaParams &p, uint32_t s, uint32_t h, uint32_t rows, uint32_t ci) {
+    const uint32_t mul = p.plan.kv_mul, row = ci / mul;
+    if (row >= rows) return ~(size_t)0;
+    return ((size_t)s * p.c.n_rows + row) * (p.c.n_head_kv * mul) + h * mul + (ci - row * mul);
+}
+
+template <class F>
+__device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
+                                      uint32_t pos0, uint32_t rows, uint32_t lane) {
+    const uint32_t col = lane & 15u, kg = lane >> 4, u = col / (16u / F::R);
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) {
+        const uint32_t ci = ct * F::COLS + n * 16u + (F::R > 1 ? col % (16u / F::R) : col);
+        const size_t head = head_of<F>(p, s, h, rows, ci);
+        const bool live   = head != ~(size_t)0;
+        const uint32_t ps = pos0 + ci / p.plan.kv_mul;
+        st.lo[n]          = live ? lfm_q4_row_lo(ps, p.plan.window) : 0u;
+        st.hi[n]          = live ? ps + 1u : 0u;
+        float x[F::G][8], big = 0.0f;
+#pragma unroll
+        for (int g = 0; g < F::G; ++g)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (live) a = reinterpret_cast<const float4 *>(p.q + head * HD)[g * 8 + kg * 2u + i];
+                if (live) a = reinterpret_cast<const float4 *>(p.q + head * F::HD)[g * 8 + kg * 2u + i];
                 x[g][4 * i] = a.x; x[g][4 * i + 1] = a.y; x[g][4 * i + 2] = a.z; x[g][4 * i + 3] = a.w;
                 big = fmaxf(big, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
             }
@@ -136,162 +200,543 @@ template <int HD> __global__ __launch_bounds__(256) void k_paged_gqa(const GqaPa
         big = fmaxf(big, __shfl_xor(big, 32));
         const int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < F::G; ++g)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y = ldexpf(x[g][i], -e);
-                qh[g][i]      = (_Float16)y;
-                ql[g][i]      = (_Float16)(y - (float)qh[g][i]);
+                const float y     = ldexpf(x[g][i], -e);
+                const _Float16 yh = (_Float16)y, yl = (_Float16)(y - (float)yh);
+#pragma unroll
+                for (int r = 0; r < F::R; ++r) {
+                    st.qh[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yh : (_Float16)0.0f;
+                    st.ql[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yl : (_Float16)0.0f;
+                }
             }
-        cs = ldexpf(p.scale * 1.4426950408889634f, e);
+        st.cs[n]  = ldexpf(p.scale * 1.4426950408889634f, e);
+        st.top[n] = st.m[n] = kNoScore;
+        st.l[n]    = 0.0f;
+        st.vmax[n] = 0u;
+#pragma unroll
+        for (int i = 0; i < F::DT; ++i) st.o[n][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
+}
 
-    float4v o[DT];
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a),
+                                                                  __builtin_bit_cast(ushort2v, b)));
+}
+
+/* One step.  EDGE: some column's rows do not attend all of its keys, or a
+ * block has no page. */
+template <class F, bool EDGE>
+__device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F> &pl, uint32_t key0, uint32_t lane) {
+    constexpr int NT = F::NT, G = F::G, J = F::J, R = F::R;
+    const uint32_t kg = lane >> 4, u = (lane & 15u) / (16u / R);
+    float sv[NT][4 * J];
+    /* S = codes . q, then s = sum over groups of scale * S, in fp32 */
 #pragma unroll
-    for (int i = 0; i < DT; ++i) o[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    float top = kNoScore, m = kNoScore, l = 0.0f;
-    uint32_t vmax = 0u; /* magnitude (fp16 bits) of the V scales that m covers */
-
-    const int32_t *table = c.table + (size_t)s * c.table_stride;
-    for (uint32_t step = t.step0; step < t.step0 + t.n_steps; ++step) {
-        const int32_t id  = table[step >> c.blk_shift];
-        const uint32_t in = step & ((1u << c.blk_shift) - 1u);
-        if ((uint32_t)id >= c.n_pages) continue; /* no page: nothing to attend */
-        const uint8_t *base = c.pages + (uint64_t)(uint32_t)id * c.page_bytes +
-                              (uint64_t)((h << c.blk_shift) + in) * lfm_q4_block_bytes(HD);
-        Block<HD> b;
-        load_block<HD>(b, base, lane);
-
-        float sv[8]; /* keys 32 step + 4 kg + i (i < 4) and 16 further */
+    for (int j = 0; j < J; ++j) {
+        float4v acc[NT][G];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float4v acc[G];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < G; ++g) acc[n][g] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = j * R + r, b = t / 2, half = t & 1;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t w = HD == 64 ? word_of(b.k[0], half * 2 + g) : word_of(b.k[half % (HD / 64)], g);
+                const uint32_t w = F::HD == 64 ? word_of(d.k[b][0], half * 2 + g) : word_of(d.k[b][half % (F::HD / 64)], g);
                 const half8v a   = unpack(w);
-                acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[g], float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[g], acc[g], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    acc[n][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.ql[n][r][g], acc[n][g], 0, 0, 0);
+                    acc[n][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.qh[n][r][g], acc[n][g], 0, 0, 0);
+                }
             }
+        }
+        const int b = J > 1 ? j / 2 : 0, w0 = J > 1 ? (j & 1) * 2 : 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x = 0.0f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const uint32_t d = word_of(b.ks[g], half * 2 + i / 2);
-                    x                = fmaf(i & 1 ? half_hi(d) : half_lo(d), acc[g][i], x);
+                    const uint32_t z = word_of(d.ks[b][g], w0 + i / 2);
+                    x                = fmaf(i & 1 ? half_hi(z) : half_lo(z), acc[n][g][i], x);
                 }
-                const uint32_t key = step * 32u + half * 16u + kg * 4u + i;
-                sv[half * 4 + i]   = key >= lo && key < hi ? x * cs : -__builtin_inff();
+                sv[n][4 * j + i] = x * st.cs[n];
+            }
+    }
+    uint4 vs[NT][J > 1 ? F::NB : 1][G];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
+#pragma unroll
+            for (int g = 0; g < G; ++g) vs[n][b][g] = d.vs[b][g];
+    if (EDGE) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const uint32_t t = J > 1 ? (uint32_t)j : u;
+                const bool page  = F::NB > 1 && (t >> 1) ? pl.there[F::NB - 1] : pl.there[0];
+                uint32_t keep[2] = {0u, 0u};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t key = key0 + 16u * t + 4u * kg + i;
+                    const bool see     = page && key >= st.lo[n] && key < st.hi[n];
+                    if (!see) sv[n][4 * j + i] = -__builtin_inff();
+                    if (see) keep[i / 2] |= i & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    uint4 &x = vs[n][J > 1 ? j / 2 : 0][g];
+                    if (J > 1 && (j & 1))
+                        x.z &= keep[0], x.w &= keep[1];
+                    else
+                        x.x &= keep[0], x.y &= keep[1];
+                }
+            }
+    }
+    float best[NT];
+    uint32_t dv[NT];
+    bool raise = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        best[n] = sv[n][0];
+        dv[n]   = 0u;
+#pragma unroll
+        for (int i = 1; i < 4 * J; ++i) best[n] = fmaxf(best[n], sv[n][i]);
+#pragma unroll
+        for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < (J > 1 ? 4 : 2); ++i)
+                    dv[n] = pk_max_u16(dv[n], word_of(vs[n][b][g], i) & 0x7FFF7FFFu);
+        dv[n] = max(dv[n] & 0xFFFFu, dv[n] >> 16);
+        raise |= best[n] > st.top[n] + kSlack || dv[n] > st.vmax[n];
+    }
+    if (__any(raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            best[n] = fmaxf(best[n], __shfl_xor(best[n], 16));
+            best[n] = fmaxf(best[n], __shfl_xor(best[n], 32));
+            dv[n]   = max(dv[n], (uint32_t)__shfl_xor((int)dv[n], 16));
+            dv[n]   = max(dv[n], (uint32_t)__shfl_xor((int)dv[n], 32));
+            st.vmax[n]    = max(dv[n], st.vmax[n]);
+            st.top[n]     = fmaxf(st.top[n], best[n]);
+            /* a scale that is not finite gives NaN in its own dims alone */
+            const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)min(st.vmax[n], 0x7BFFu));
+            const float m = st.top[n] + (x > 0.0f ? (float)__builtin_amdgcn_frexp_expf(x) : 0.0f) - kLift;
+            const float a = __builtin_amdgcn_exp2f(st.m[n] - m);
+            st.l[n] *= a;
+#pragma unroll
+            for (int i = 0; i < F::DT; ++i) st.o[n][i] *= a;
+            st.m[n] = m;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) {
+            sv[n][i] = __builtin_amdgcn_exp2f(sv[n][i] - st.m[n]);
+            st.l[n] += sv[n][i];
+        }
+    /* O += codes . (p * scale), per block and group of dims */
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        uint32_t ch[2], cl[2]; /* R > 1: this lane's 4 keys */
+        if constexpr (R > 1) {
+            const uint4 z = vs[0][0][g];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t w = i ? z.y : z.x;
+                const float a = sv[0][2 * i] * half_lo(w), c = sv[0][2 * i + 1] * half_hi(w);
+                ch[i] = pk_rtz(a, c);
+                cl[i] = pk_rtz(a - half_lo(ch[i]), c - half_hi(ch[i]));
             }
         }
-        float best = sv[0];
-        uint32_t dv = 0u;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) best = fmaxf(best, sv[i]);
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t d = (word_of(b.vs[g], i / 2) >> (16 * (i & 1))) & 0x7FFFu;
-                dv               = max(dv, sv[i] > -__builtin_inff() && d < 0x7C00u ? d : 0u);
-            }
-        if (__any(best > top + kSlack || dv > vmax)) {
-            best = fmaxf(best, __shfl_xor(best, 16));
-            best = fmaxf(best, __shfl_xor(best, 32));
-            dv   = max(dv, (uint32_t)__shfl_xor((int)dv, 16));
-            dv   = max(dv, (uint32_t)__shfl_xor((int)dv, 32));
-            vmax = max(dv, vmax);
-            top  = fmaxf(top, best);
-            const float d = (float)__builtin_bit_cast(_Float16, (uint16_t)vmax);
-            const float n = top + (d > 0.0f ? (float)__builtin_amdgcn_frexp_expf(d) : 0.0f) - kLift;
-            const float a = __builtin_amdgcn_exp2f(m - n);
-            l *= a;
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] *= a;
-            m = n;
-        }
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            pr[i] = __builtin_amdgcn_exp2f(sv[i] - m);
-            l += pr[i];
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int b = 0; b < F::NB; ++b) {
             union {
                 uint32_t u[4];
                 half8v v;
-            } wh, wl;
+            } wh[NT], wl[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t d = word_of(b.vs[g], i);
-                const float a = sv[2 * i] > -__builtin_inff() ? pr[2 * i] * half_lo(d) : 0.0f;
-                const float z = sv[2 * i + 1] > -__builtin_inff() ? pr[2 * i + 1] * half_hi(d) : 0.0f;
-                wh.u[i]       = pk_rtz(a, z);
-                wl.u[i]       = pk_rtz(a - half_lo(wh.u[i]), z - half_hi(wh.u[i]));
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (R > 1) {
+                        const bool mine = u == (uint32_t)((2 * b + i / 2) % R);
+                        wh[n].u[i]      = mine ? ch[i & 1] : 0u;
+                        wl[n].u[i]      = mine ? cl[i & 1] : 0u;
+                    } else {
+                        const uint32_t w = word_of(vs[n][b][g], i);
+                        const float a = sv[n][8 * b + 2 * i] * half_lo(w), c = sv[n][8 * b + 2 * i + 1] * half_hi(w);
+                        wh[n].u[i] = pk_rtz(a, c);
+                        wl[n].u[i] = pk_rtz(a - half_lo(wh[n].u[i]), c - half_hi(wh[n].u[i]));
+                    }
+                }
 #pragma unroll
             for (int i = 2 * g; i < 2 * g + 2; ++i) {
-                const half8v a = unpack(word_of(b.v[i / 4], i & 3));
-                o[i]           = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl.v, o[i], 0, 0, 0);
-                o[i]           = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh.v, o[i], 0, 0, 0);
+                const half8v a = unpack(word_of(d.v[b][i / 4], i & 3));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    st.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[n].v, st.o[n][i], 0, 0, 0);
+                    st.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[n].v, st.o[n][i], 0, 0, 0);
+                }
             }
         }
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (!live) return;
-    float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); /* no key: 0; NaN stays */
+}
+
+/* Steps [a, b) of unit (s, ct, h): loads run one step ahead, table entries two. */
+template <class F>
+__device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t h,
+                                          const lfm_q4_tile &t, uint32_t pos0, uint32_t a, uint32_t b, uint32_t lane) {
+    const int32_t *table = p.c.table + (size_t)s * p.c.table_stride;
+    /* keys that every row of the tile attends */
+    const uint32_t in0 = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window), in1 = pos0 + t.r0 + 1u;
+    Place<F> at = place_of<F>(p.c, table, h, a);
+    Step<F> d;
+    load_step<F>(d, at, lane);
+    Place<F> next = place_of<F>(p.c, table, h, a + 1u < b ? a + 1u : a);
+    for (uint32_t step = a; step < b; ++step) {
+        Step<F> e;
+        load_step<F>(e, next, lane);
+        const Place<F> after = place_of<F>(p.c, table, h, step + 2u < b ? step + 2u : b - 1u);
+        const uint32_t key0  = step * F::STEP;
+        bool inner           = key0 >= in0 && key0 + F::STEP <= in1;
+#pragma unroll
+        for (int i = 0; i < F::NB; ++i) inner = inner && at.there[i];
+        if (inner)
+            run_step<F, false>(st, d, at, key0, lane);
+        else
+            run_step<F, true>(st, d, at, key0, lane);
+        d    = e;
+        at   = next;
+        next = after;
+    }
+}
+
+/* Sums over the lanes that share a column; with R > 1 its copies too. */
+template <class F> __device__ __forceinline__ void join_lanes(State<F> &st) {
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) {
+        st.l[n] += __shfl_xor(st.l[n], 16);
+        st.l[n] += __shfl_xor(st.l[n], 32);
+    }
+    if constexpr (F::R > 1) {
+        float m = st.m[0];
+#pragma unroll
+        for (int x = 16 / F::R; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
+        const float a = __builtin_amdgcn_exp2f(st.m[0] - m);
+        st.l[0] *= a;
+#pragma unroll
+        for (int i = 0; i < F::DT; ++i) st.o[0][i] *= a;
+#pragma unroll
+        for (int x = 16 / F::R; x < 16; x *= 2) {
+            st.l[0] += __shfl_xor(st.l[0], x);
+#pragma unroll
+            for (int i = 0; i < F::DT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.o[0][i][k] += __shfl_xor(st.o[0][i][k], x);
+        }
+        st.m[0] = m;
+    }
+}
+
+/* 1 / l (0 where no key was attended, NaN where a score was) times the gate. */
+__device__ __forceinline__ float out_factor(const GqaParams &p, float l, size_t head) {
+    float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
     if (p.gate) {
         const float x = p.gate[head];
         f *= p.gate_is_logit ? 1.0f / (1.0f + expf(-x)) : x;
     }
+    return f;
+}
+
+template <class F>
+__device__ __forceinline__ void write_out(const State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
+                                          uint32_t rows, uint32_t lane) {
+    const uint32_t col = lane & 15u, kg = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-        reinterpret_cast<float4 *>(p.out + head * HD)[i * 4 + kg] =
-            make_float4(o[i][0] * f, o[i][1] * f, o[i][2] * f, o[i][3] * f);
+    for (int n = 0; n < F::NT; ++n) {
+        if (F::R > 1 && col >= 16u / F::R) continue;
+        const size_t head = head_of<F>(p, s, h, rows, ct * F::COLS + n * 16u + col);
+        if (head == ~(size_t)0) continue;
+        const float f = out_factor(p, st.l[n], head);
+#pragma unroll
+        for (int i = 0; i < F::DT; ++i)
+            reinterpret_cast<float4 *>(p.out + head * F::HD)[i * 4 + kg] =
+                make_float4(st.o[n][i][0] * f, st.o[n][i][1] * f, st.o[n][i][2] * f, st.o[n][i][3] * f);
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void write_part(const State<F> &st, const GqaParams &p, uint64_t slot, uint32_t lane) {
+    const uint32_t col = lane & 15u, kg = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) {
+        if (F::R > 1 && col >= 16u / F::R) continue;
+        const size_t at = (size_t)slot * F::COLS + n * 16u + col;
+        if (kg == 0u) p.part_ml[at] = make_float2(st.m[n], st.l[n]);
+#pragma unroll
+        for (int i = 0; i < F::DT; ++i)
+            reinterpret_cast<float4 *>(p.part_o + at * F::HD)[i * 4 + kg] =
+                make_float4(st.o[n][i][0], st.o[n][i][1], st.o[n][i][2], st.o[n][i][3]);
+    }
+}
+
+__device__ __forceinline__ uint32_t rows_of(const PagedQ4 &c, uint32_t s, uint32_t pos0) {
+    return lfm_q4_rows(pos0, c.rows_seq ? c.rows_seq[s] : c.n_rows, c.n_rows, c.capacity);
+}
+
+/* Every wave one unit, all its keys. */
+template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa(const GqaParams p) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t unit = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
+    const uint32_t h = unit % p.c.n_head_kv, sc = unit / p.c.n_head_kv;
+    const uint32_t s = sc / p.plan.n_ct, ct = sc - s * p.plan.n_ct;
+    if (s >= p.c.n_seq) return;
+    const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
+    const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
+    if (t.n_steps == 0u) return;
+    State<F> st;
+    start<F>(st, p, s, ct, h, pos0, rows, lane);
+    run_piece<F>(st, p, s, h, t, pos0, t.step0, t.step0 + t.n_steps, lane);
+    join_lanes<F>(st);
+    write_out<F>(st, p, s, ct, h, rows, lane);
+}
+
+/* Steps of entry e (sequence, tile), 0 past the last. */
+__device__ __forceinline__ uint32_t entry_steps(const GqaParams &p, uint32_t e, uint32_t n_entries) {
+    if (e >= n_entries) return 0u;
+    const uint32_t s = e / p.plan.n_ct, pos0 = p.c.pos0[s];
+    return lfm_q4_tile_of(&p.plan, pos0, rows_of(p.c, s, pos0), e - s * p.plan.n_ct).n_steps;
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t lane) { /* inclusive */
+#pragma unroll
+    for (uint32_t o = 1; o < 64u; o *= 2u) {
+        const uint32_t y = (uint32_t)__shfl_up((int)x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+/* Equal shares of the batch's steps per wave. */
+template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(const GqaParams p) {
+    const uint32_t lane = threadIdx.x & 63u, nh = p.c.n_head_kv;
+    const uint32_t wave = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
+    const uint32_t n_e  = p.c.n_seq * p.plan.n_ct;
+    uint32_t total = 0u;
+    for (uint32_t e0 = 0; e0 < n_e; e0 += 64u) {
+        const uint32_t inc = wave_scan(entry_steps(p, e0 + lane, n_e), lane);
+        if (wave == 0u && e0 + lane < n_e) p.pre[e0 + lane + 1u] = total + inc;
+        total += uniform((uint32_t)__shfl((int)inc, 63));
+    }
+    if (wave == 0u && lane == 0u) p.pre[0] = 0u;
+    const uint64_t N = (uint64_t)total * nh;
+    if (N == 0u) return;
+    const uint32_t G = lfm_q4_waves(&p.plan, N);
+    if (wave >= G) return;
+    uint64_t t        = lfm_q4_share(wave, N, G);
+    const uint64_t t1 = lfm_q4_share(wave + 1u, N, G);
+    /* the entry holding step t */
+    uint32_t e = 0u, before = 0u, want = (uint32_t)(t / nh);
+    for (uint32_t e0 = 0;; e0 += 64u) {
+        const uint32_t n = entry_steps(p, e0 + lane, n_e), inc = wave_scan(n, lane);
+        const uint64_t hit = __ballot(before + inc > want);
+        if (hit) {
+            const int i = __builtin_ctzll(hit);
+            e           = e0 + (uint32_t)i;
+            before += uniform((uint32_t)__shfl((int)(inc - n), i));
+            break;
+        }
+        before += uniform((uint32_t)__shfl((int)inc, 63));
+    }
+    e = uniform(e);
+    while (t < t1) {
+        const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
+        const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
+        const lfm_q4_tile tile = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
+        const uint64_t first   = (uint64_t)before * nh;
+        while (t < t1 && t < first + (uint64_t)tile.n_steps * nh) {
+            const uint32_t h  = uniform((uint32_t)((t - first) / tile.n_steps));
+            const uint64_t u0 = first + (uint64_t)h * tile.n_steps;
+            const uint64_t u1 = u0 + tile.n_steps;
+            const uint64_t te = t1 < u1 ? t1 : u1;
+            const uint32_t a = uniform((uint32_t)(t - u0)), b = uniform((uint32_t)(te - u0));
+            State<F> st;
+            start<F>(st, p, s, ct, h, pos0, rows, lane);
+            run_piece<F>(st, p, s, h, tile, pos0, tile.step0 + a, tile.step0 + b, lane);
+            join_lanes<F>(st);
+            if (a == 0u && b == tile.n_steps)
+                write_out<F>(st, p, s, ct, h, rows, lane);
+            else
+                write_part<F>(st, p, (uint64_t)wave + (uint64_t)e * nh + h, lane);
+            t = te;
+        }
+        before += tile.n_steps;
+        ++e;
+    }
+}
+
+/* The pieces of every unit that more than one wave holds: one workgroup per
+ * (unit, column); HD / 4 threads take a piece, 1024 / HD pieces at a time. */
+template <int HD> __global__ __launch_bounds__(256) void k_paged_merge(const GqaParams p) {
+    constexpr uint32_t L = HD / 4, P = 256u / L;
+    __shared__ float sm[P], sl[P];
+    __shared__ float4 so[P][L];
+    const uint32_t nh = p.c.n_head_kv, cols = p.plan.cols;
+    const uint32_t unit = blockIdx.x / cols, col = blockIdx.x - unit * cols;
+    const uint32_t e = unit / nh, h = unit - e * nh;
+    const uint32_t n = p.pre[e + 1u] - p.pre[e];
+    if (n == 0u) return;
+    const uint64_t N = (uint64_t)p.pre[p.c.n_seq * p.plan.n_ct] * nh, first = (uint64_t)p.pre[e] * nh + (uint64_t)h * n;
+    const uint32_t G = lfm_q4_waves(&p.plan, N);
+    const uint32_t g0 = lfm_q4_owner(first, N, G), g1 = lfm_q4_owner(first + n - 1u, N, G);
+    if (g0 == g1) return;
+    const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
+    const uint32_t rows = rows_of(p.c, s, p.c.pos0[s]);
+    const uint32_t mul = p.plan.kv_mul, ci = ct * cols + col, row = ci / mul;
+    if (row >= rows) return;
+    const size_t head = ((size_t)s * p.c.n_rows + row) * (nh * mul) + h * mul + (ci - row * mul);
+    const uint32_t i = threadIdx.x % L, k = threadIdx.x / L;
+    float m = kNoScore, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t g = g0 + k; g <= g1; g += P) {
+        const size_t at = ((size_t)g + unit) * cols + col;
+        const float2 ml = p.part_ml[at];
+        const float4 x  = reinterpret_cast<const float4 *>(p.part_o + at * HD)[i];
+        const float mn = fmaxf(m, ml.x), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(ml.x - mn);
+        m = mn;
+        l = l * a + ml.y * b;
+        o = make_float4(o.x * a + x.x * b, o.y * a + x.y * b, o.z * a + x.z * b, o.w * a + x.w * b);
+    }
+    so[k][i] = o;
+    if (i == 0u) sm[k] = m, sl[k] = l;
+    __syncthreads();
+    if (k != 0u) return;
+    float mm = m;
+#pragma unroll
+    for (uint32_t j = 1; j < P; ++j) mm = fmaxf(mm, sm[j]);
+    float ll = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t j = 0; j < P; ++j) {
+        const float b = __builtin_amdgcn_exp2f(sm[j] - mm);
+        const float4 x = so[j][i];
+        ll += sl[j] * b;
+        o = make_float4(o.x + x.x * b, o.y + x.y * b, o.z + x.z * b, o.w + x.w * b);
+    }
+    const float f = out_factor(p, ll, head);
+    reinterpret_cast<float4 *>(p.out + head * HD)[i] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+}
+
+/* ---- host: forms, split, scratch ------------------------------------------------ */
+constexpr uint32_t kWaves = 2048u; /* two per SIMD of 256 compute units */
+
+struct Launch {
+    lfm_q4_plan plan;
+    uint32_t copies, tiles; /* R and NT of the form */
+    bool split;
+    size_t o_bytes, ml_bytes, pre_bytes;
+};
+
+int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
+                uint32_t head_dim, uint32_t capacity, uint32_t window) {
+    lfm_q4_plan &p      = L->plan;
+    const uint32_t mul  = n_head_q / n_head_kv;
+    const uint64_t cols = (uint64_t)n_rows * mul;
+    if (cols > 0x7FFFFFFFull) return LFM_ATTN_E_UNSUPPORTED;
+    p.n_seq     = n_seq;
+    p.n_rows    = n_rows;
+    p.kv_mul    = mul;
+    p.n_head_kv = n_head_kv;
+    p.window    = window;
+    p.capacity  = capacity;
+    L->tiles    = 1u;
+    L->copies   = 1u;
+    if (head_dim == 64u && cols <= 4u) L->copies = 4u;
+    if (head_dim == 128u && cols <= 8u) L->copies = 2u;
+    p.cols = L->copies > 1u ? 16u / L->copies : 16u * L->tiles;
+    p.step = L->copies == 4u ? 64u : 32u;
+    p.n_ct = (uint32_t)((cols + p.cols - 1u) / p.cols);
+    p.min_steps = 1u;
+    const uint64_t entries = (uint64_t)n_seq * p.n_ct, units = entries * n_head_kv;
+    if (units > 0x7FFFFFFFull / p.cols) return LFM_ATTN_E_UNSUPPORTED;
+    uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
+    if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
+    const uint64_t steps = (keys + p.step - 1u) / p.step + (window ? 1u : 0u);
+    /* enough units fill the card by themselves; step counts of a split are 32 bits */
+    L->split = units < 2u * kWaves && entries * (capacity / 32u) < 0xFFFFFFFFull;
+    uint64_t waves = units * steps / p.min_steps;
+    if (waves > kWaves) waves = kWaves;
+    p.n_waves    = (uint32_t)((waves + 3u) / 4u * 4u);
+    const uint64_t slots = L->split ? p.n_waves + units : 0u;
+    L->o_bytes   = slots * p.cols * head_dim * 4u;
+    L->ml_bytes  = slots * p.cols * 8u;
+    L->pre_bytes = L->split ? (entries + 1u) * 4u : 0u;
+    return LFM_ATTN_OK;
+}
+
+template <class F> void launch_form(const GqaParams &p, bool split, hipStream_t stream) {
+    const uint64_t units = (uint64_t)p.c.n_seq * p.plan.n_ct * p.c.n_head_kv;
+    if (split) {
+        hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(k_paged_merge<F::HD>, dim3((uint32_t)(units * p.plan.cols)), dim3(256), 0, stream, p);
+    } else {
+        hipLaunchKernelGGL(k_paged_gqa<F>, dim3((uint32_t)((units + 3u) / 4u)), dim3(256), 0, stream, p);
+    }
 }
 
 } // namespace
 
 int paged_q4_gqa_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
                            uint32_t head_dim, uint32_t capacity, uint32_t window, size_t *bytes) {
-    (void)keys_hint, (void)head_dim, (void)capacity, (void)window;
-    const uint64_t cols = (uint64_t)n_rows * (n_head_q / n_head_kv);
-    if (cols > 0x7FFFFFFFull || (cols + 15u) / 16u * n_seq > 0x7FFFFFFFull / n_head_kv) return LFM_ATTN_E_UNSUPPORTED;
-    *bytes = 0;
+    Launch L;
+    const int st = plan_launch(&L, n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, capacity, window);
+    if (st != LFM_ATTN_OK) return st;
+    *bytes = L.o_bytes + L.ml_bytes + L.pre_bytes;
     return LFM_ATTN_OK;
 }
 
 int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int gate_is_logit, float *out,
                         uint32_t n_head_q, uint32_t keys_hint, uint32_t window, float scale, void *workspace,
                         hipStream_t stream) {
-    (void)keys_hint, (void)workspace;
+    Launch L;
+    const int st =
+        plan_launch(&L, c.n_seq, c.n_rows, keys_hint, n_head_q, c.n_head_kv, c.head_dim, c.capacity, window);
+    if (st != LFM_ATTN_OK) return st;
     GqaParams p;
-    p.c              = c;
-    p.plan.n_seq     = c.n_seq;
-    p.plan.n_rows    = c.n_rows;
-    p.plan.kv_mul    = n_head_q / c.n_head_kv;
-    p.plan.n_head_kv = c.n_head_kv;
-    p.plan.window    = window;
-    p.plan.capacity  = c.capacity;
-    p.plan.cols      = 16u;
-    p.plan.step      = 32u;
-    p.plan.n_ct      = (c.n_rows * p.plan.kv_mul + 15u) / 16u;
-    p.plan.min_steps = 1u;
-    p.plan.n_waves   = 0u;
-    p.q              = q;
-    p.gate           = gate;
-    p.out            = out;
-    p.gate_is_logit  = gate_is_logit;
-    p.scale          = scale;
-    const uint64_t units = (uint64_t)c.n_seq * p.plan.n_ct * c.n_head_kv;
-    const dim3 grid((uint32_t)((units + 3u) / 4u));
-    if (c.head_dim == 64u)
-        hipLaunchKernelGGL(k_paged_gqa<64>, grid, dim3(256), 0, stream, p);
-    else
-        hipLaunchKernelGGL(k_paged_gqa<128>, grid, dim3(256), 0, stream, p);
+    p.c             = c;
+    p.plan          = L.plan;
+    p.q             = q;
+    p.gate          = gate;
+    p.out           = out;
+    p.gate_is_logit = gate_is_logit;
+    p.scale         = scale;
+    uint8_t *w      = static_cast<uint8_t *>(workspace);
+    p.part_o        = reinterpret_cast<float *>(w);
+    p.part_ml       = reinterpret_cast<float2 *>(w + L.o_bytes);
+    p.pre           = reinterpret_cast<uint32_t *>(w + L.o_bytes + L.ml_bytes);
+    if (c.head_dim == 64u) {
+        if (L.copies == 4u)
+            launch_form<Form<64, 1, 4, 2>>(p, L.split, stream);
+        else
+            launch_form<Form<64, 1, 1, 1>>(p, L.split, stream);
+    } else {
+        if (L.copies == 2u)
+            launch_form<Form<128, 1, 2, 1>>(p, L.split, stream);
+        else
+            launch_form<Form<128, 1, 1, 1>>(p, L.split, stream);
+    }
     return hip_status(hipGetLastError());
 }
 
