@@ -43,33 +43,63 @@ struct GqaParams {
     float *out;
     int gate_is_logit;
     float scale;
-    /* split: steps before each entry (sequence, tile) and in all [n_entries + 1],
-     * partial outputs [slot][cols][HD], their (m, l) [slot][cols] */
-    uint32_t *pre;
+    /* split: first and last wave of each unit, partial outputs
+     * [slot][cols][HD], their (m, l) [slot][cols] */
+    uint2 *range;
     float *part_o;
     float2 *part_ml;
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
-/* The 8 codes of a word as the A operand of one MFMA, exact: code - 8. */
-__device__ __forceinline__ half8v unpack(uint32_t w) {
-    union {
-        uint32_t u[4];
-        half2v h[4];
-        half8v v;
-    } r;
+/* Constants of the unpacking in vector registers: an and-or takes one scalar operand. */
+struct Magic {
+    uint32_t b1024, b64;
+};
+__device__ __forceinline__ Magic magic() {
+    Magic m;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(m.b1024));
+    asm("v_mov_b32 %0, 0x54005400" : "=v"(m.b64));
+    return m;
+}
+
+union Words {
+    uint32_t u[4];
+    half2v h[4];
+    half8v v;
+};
+
+/* The 8 codes of a V word as the A operand of one MFMA, exact: code - 8. */
+__device__ __forceinline__ half8v unpack_v(uint32_t w, const Magic &k) {
+    Words r;
     const half2v b0 = {(_Float16)-1032.0f, (_Float16)-1032.0f};
     const half2v s1 = {(_Float16)0.0625f, (_Float16)0.0625f}, b1 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const uint32_t x = w >> 8;
-    r.u[0] = (w & 0x000F000Fu) | 0x64006400u; /* 1024 + code      */
-    r.u[1] = (w & 0x00F000F0u) | 0x64006400u; /* 1024 + 16 * code */
-    r.u[2] = (x & 0x000F000Fu) | 0x64006400u;
-    r.u[3] = (x & 0x00F000F0u) | 0x64006400u;
+    r.u[0] = (w & 0x000F000Fu) | k.b1024; /* 1024 + code      */
+    r.u[1] = (w & 0x00F000F0u) | k.b1024; /* 1024 + 16 * code */
+    r.u[2] = (x & 0x000F000Fu) | k.b1024;
+    r.u[3] = (x & 0x00F000F0u) | k.b1024;
     r.h[0] = r.h[0] + b0;
     r.h[1] = __builtin_elementwise_fma(r.h[1], s1, b1);
     r.h[2] = r.h[2] + b0;
     r.h[3] = __builtin_elementwise_fma(r.h[3], s1, b1);
+    return r.v;
+}
+
+/* A K word: elements 0, 1, 4, 5 as code - 8, elements 2, 3, 6, 7 as code + 64.
+ * The product with q starts from -72 times the sum of q over the latter, so it
+ * is that of code - 8; at 9 times the codes' size fp32 still has bits to spare,
+ * which the values' long sums would not have. */
+__device__ __forceinline__ half8v unpack_k(uint32_t w, const Magic &k) {
+    Words r;
+    const half2v b0  = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    const uint32_t x = w >> 8;
+    r.u[0] = (w & 0x000F000Fu) | k.b1024;
+    r.u[1] = (w & 0x00F000F0u) | k.b64;
+    r.u[2] = (x & 0x000F000Fu) | k.b1024;
+    r.u[3] = (x & 0x00F000F0u) | k.b64;
+    r.h[0] = r.h[0] + b0;
+    r.h[2] = r.h[2] + b0;
     return r.v;
 }
 
@@ -97,62 +127,67 @@ template <int HD_, int NT_, int R_, int NB_> struct Form {
     static_assert(R == 1 || (NT == 1 && J == 1), "a copy takes one tile per step");
 };
 
-template <class F> struct Step { /* one lane's share of a step's codes and scales */
-    uint4 k[F::NB][F::HD / 64], v[F::NB][F::HD / 64];
-    uint4 ks[F::J > 1 ? F::NB : 1][F::G], vs[F::J > 1 ? F::NB : 1][F::G]; /* J 1: .x and .y alone */
+/* One lane's share of a step's codes and scales, keys or values. */
+template <class F> struct Half {
+    uint4 c[F::NB][F::HD / 64];
+    uint4 s[F::J > 1 ? F::NB : 1][F::G]; /* J 1: .x and .y alone */
 };
 
-/* Wave-uniform place of a step: its blocks, and whether they have pages. */
-template <class F> struct Place {
-    const uint8_t *base[F::NB];
-    bool there[F::NB];
+/* Wave-uniform place of a step: its one or two blocks, and whether they have
+ * pages.  (Members rather than arrays: an array that lanes index moves to LDS.) */
+struct Place {
+    const uint8_t *base0, *base1;
+    bool there0, there1;
 };
 
-template <class F>
-__device__ __forceinline__ Place<F> place_of(const PagedQ4 &c, const int32_t *table, uint32_t h, uint32_t step) {
-    Place<F> p;
-#pragma unroll
-    for (int b = 0; b < F::NB; ++b) {
-        /* a step's last block may lie behind the table: its keys are masked, read the one before */
-        uint32_t blk = step * F::NB + b;
-        if (F::NB > 1 && blk * 32u >= c.capacity) blk = c.capacity / 32u - 1u;
-        const int32_t id  = table[blk >> c.blk_shift];
-        const uint32_t in = blk & ((1u << c.blk_shift) - 1u);
-        p.there[b]        = (uint32_t)id < c.n_pages;
-        p.base[b]         = c.pages + (uint64_t)(p.there[b] ? (uint32_t)id : 0u) * c.page_bytes +
-                    (uint64_t)((h << c.blk_shift) + in) * lfm_q4_block_bytes(F::HD);
+/* The table through the scalar cache: no kernel that runs beside this one writes it. */
+typedef const __attribute__((address_space(4))) int32_t *TableRow;
+
+__device__ __forceinline__ bool block_place(const PagedQ4 &c, TableRow table, uint32_t h, uint32_t blk,
+                                            uint32_t block_bytes, const uint8_t **base) {
+    const uint32_t id = (uint32_t)table[blk >> c.blk_shift], in = blk & ((1u << c.blk_shift) - 1u);
+    const bool there  = id < c.n_pages;
+    *base = c.pages + (uint64_t)(there ? id : 0u) * c.page_bytes + (uint64_t)(((h << c.blk_shift) + in) * block_bytes);
+    return there;
+}
+
+template <class F> __device__ __forceinline__ Place place_of(const PagedQ4 &c, TableRow table, uint32_t h, uint32_t step) {
+    Place p;
+    p.there0 = block_place(c, table, h, step * F::NB, 36u * F::HD, &p.base0);
+    p.there1 = p.there0;
+    p.base1  = p.base0;
+    if (F::NB > 1) { /* a step's last block may lie behind the table: its keys are masked, read the first twice */
+        const uint32_t blk = step * F::NB + 1u;
+        p.there1 = block_place(c, table, h, blk * 32u < c.capacity ? blk : blk - 1u, 36u * F::HD, &p.base1);
     }
     return p;
 }
 
-template <class F> __device__ __forceinline__ void load_step(Step<F> &d, const Place<F> &p, uint32_t lane) {
+/* V 0: keys, 1: values. */
+template <class F, int V> __device__ __forceinline__ void load_half(Half<F> &d, const Place &p, uint32_t lane) {
     constexpr int HD = F::HD;
     const uint32_t kg = lane >> 4;
 #pragma unroll
     for (int b = 0; b < F::NB; ++b)
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) {
-            d.k[b][i] = *reinterpret_cast<const uint4 *>(p.base[b] + i * 1024 + lane * 16u);
-            d.v[b][i] = *reinterpret_cast<const uint4 *>(p.base[b] + 16 * HD + i * 1024 + lane * 16u);
-        }
+        for (int i = 0; i < HD / 64; ++i)
+            d.c[b][i] = *reinterpret_cast<const uint4 *>((b ? p.base1 : p.base0) + V * 16 * HD + i * 1024 + lane * 16u);
     if constexpr (F::J > 1) {
 #pragma unroll
         for (int b = 0; b < F::NB; ++b)
 #pragma unroll
-            for (int g = 0; g < F::G; ++g) {
-                d.ks[b][g] = *reinterpret_cast<const uint4 *>(p.base[b] + 32 * HD + g * 64 + kg * 16u);
-                d.vs[b][g] = *reinterpret_cast<const uint4 *>(p.base[b] + 34 * HD + g * 64 + kg * 16u);
-            }
+            for (int g = 0; g < F::G; ++g)
+                d.s[b][g] =
+                    *reinterpret_cast<const uint4 *>((b ? p.base1 : p.base0) + (32 + 2 * V) * HD + g * 64 +
+                                                     kg * 16u);
     } else { /* the 4 keys of this lane's tile */
         const uint32_t u    = (lane & 15u) / (16u / F::R);
-        const uint8_t *base = F::NB > 1 && (u >> 1) ? p.base[F::NB - 1] : p.base[0];
-        base += 32 * HD + kg * 16u + (u & 1u) * 8u;
+        const int64_t other = F::NB > 1 ? -(int64_t)(u >> 1) & (p.base1 - p.base0) : 0;
+        const uint8_t *base = p.base0 + other + ((32 + 2 * V) * HD + kg * 16u + (u & 1u) * 8u);
 #pragma unroll
         for (int g = 0; g < F::G; ++g) {
             const uint2 a = *reinterpret_cast<const uint2 *>(base + g * 64);
-            const uint2 z = *reinterpret_cast<const uint2 *>(base + 2 * HD + g * 64);
-            d.ks[0][g]    = make_uint4(a.x, a.y, 0u, 0u);
-            d.vs[0][g]    = make_uint4(z.x, z.y, 0u, 0u);
+            d.s[0][g]     = make_uint4(a.x, a.y, 0u, 0u);
         }
     }
 }
@@ -161,8 +196,9 @@ template <class F> __device__ __forceinline__ void load_step(Step<F> &d, const P
 template <class F> struct State {
     half8v qh[F::NT][F::R][F::G], ql[F::NT][F::R][F::G];
     float4v o[F::NT][F::DT];
+    float c0[F::NT][F::G];           /* start of the S product: minus 72 sum q (unpack_k) */
     float cs[F::NT], top[F::NT], m[F::NT], l[F::NT];
-    uint32_t vmax[F::NT];            /* magnitude (fp16 bits) of the V scales that m covers */
+    uint32_t vmax;                   /* magnitude (fp16 bits) of the V scales that m covers */
     uint32_t lo[F::NT], hi[F::NT];   /* keys [lo, hi) of the column's row */
 };
 
@@ -200,21 +236,28 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
         big = fmaxf(big, __shfl_xor(big, 32));
         const int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
-        for (int g = 0; g < F::G; ++g)
+        for (int g = 0; g < F::G; ++g) {
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y     = ldexpf(x[g][i], -e);
+                const float y     = ldexpf(p.scale < 0.0f ? -x[g][i] : x[g][i], -e);
                 const _Float16 yh = (_Float16)y, yl = (_Float16)(y - (float)yh);
+                if (i & 2) sum += (float)yh + (float)yl;
 #pragma unroll
                 for (int r = 0; r < F::R; ++r) {
                     st.qh[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yh : (_Float16)0.0f;
                     st.ql[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yl : (_Float16)0.0f;
                 }
             }
-        st.cs[n]  = ldexpf(p.scale * 1.4426950408889634f, e);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            st.c0[n][g] = -72.0f * sum;
+        }
+        /* never 0: a masked score is cs * -inf */
+        st.cs[n]  = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e), 1e-37f);
         st.top[n] = st.m[n] = kNoScore;
-        st.l[n]    = 0.0f;
-        st.vmax[n] = 0u;
+        st.l[n] = 0.0f;
+        st.vmax = 0u;
 #pragma unroll
         for (int i = 0; i < F::DT; ++i) st.o[n][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -226,28 +269,27 @@ __device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
                                                                   __builtin_bit_cast(ushort2v, b)));
 }
 
-/* One step.  EDGE: some column's rows do not attend all of its keys, or a
- * block has no page. */
-template <class F, bool EDGE>
-__device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F> &pl, uint32_t key0, uint32_t lane) {
+/* Scores of a step before the factor cs: sum over groups of scale * (codes . q). */
+template <class F>
+__device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<F> &st, const Half<F> &k,
+                                       const Magic &mg) {
     constexpr int NT = F::NT, G = F::G, J = F::J, R = F::R;
-    const uint32_t kg = lane >> 4, u = (lane & 15u) / (16u / R);
-    float sv[NT][4 * J];
-    /* S = codes . q, then s = sum over groups of scale * S, in fp32 */
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         float4v acc[NT][G];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int g = 0; g < G; ++g) acc[n][g] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int g = 0; g < G; ++g)
+                acc[n][g] = float4v{st.c0[n][g], st.c0[n][g], st.c0[n][g], st.c0[n][g]};
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int t = j * R + r, b = t / 2, half = t & 1;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t w = F::HD == 64 ? word_of(d.k[b][0], half * 2 + g) : word_of(d.k[b][half % (F::HD / 64)], g);
-                const half8v a   = unpack(w);
+                const uint32_t w =
+                    F::HD == 64 ? word_of(k.c[b][0], half * 2 + g) : word_of(k.c[b][half % (F::HD / 64)], g);
+                const half8v a = unpack_k(w, mg);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     acc[n][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.ql[n][r][g], acc[n][g], 0, 0, 0);
@@ -260,78 +302,89 @@ __device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = 0.0f;
+                float y = 0.0f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const uint32_t z = word_of(d.ks[b][g], w0 + i / 2);
-                    x                = fmaf(i & 1 ? half_hi(z) : half_lo(z), acc[n][g][i], x);
+                    const uint32_t z = word_of(k.s[b][g], w0 + i / 2);
+                    y                = fmaf(i & 1 ? half_hi(z) : half_lo(z), acc[n][g][i], y);
                 }
-                sv[n][4 * j + i] = x * st.cs[n];
+                x[n][4 * j + i] = y;
             }
     }
-    uint4 vs[NT][J > 1 ? F::NB : 1][G];
+}
+
+/* A step that some row does not attend whole, or with a block that has no
+ * page: masked scores become -inf, V scales that no column of the lane needs
+ * 0 (weights of masked keys are then 0 whatever was stored). */
+template <class F>
+__device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &v, const State<F> &st,
+                                          const Place &pl, uint32_t key0, uint32_t lane) {
+    constexpr int NT = F::NT, G = F::G, J = F::J;
+    const uint32_t kg = lane >> 4, u = (lane & 15u) / (16u / F::R);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int j = 0; j < J; ++j) {
+        const uint32_t t = J > 1 ? (uint32_t)j : u;
+        const bool page  = (pl.there0 || t >= 2u) && (pl.there1 || t < 2u);
+        uint32_t keep[2] = {0u, 0u};
 #pragma unroll
-        for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t key = key0 + 16u * t + 4u * kg + i;
+            bool any           = false;
 #pragma unroll
-            for (int g = 0; g < G; ++g) vs[n][b][g] = d.vs[b][g];
-    if (EDGE) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const uint32_t t = J > 1 ? (uint32_t)j : u;
-                const bool page  = F::NB > 1 && (t >> 1) ? pl.there[F::NB - 1] : pl.there[0];
-                uint32_t keep[2] = {0u, 0u};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t key = key0 + 16u * t + 4u * kg + i;
-                    const bool see     = page && key >= st.lo[n] && key < st.hi[n];
-                    if (!see) sv[n][4 * j + i] = -__builtin_inff();
-                    if (see) keep[i / 2] |= i & 1 ? 0xFFFF0000u : 0x0000FFFFu;
-                }
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    uint4 &x = vs[n][J > 1 ? j / 2 : 0][g];
-                    if (J > 1 && (j & 1))
-                        x.z &= keep[0], x.w &= keep[1];
-                    else
-                        x.x &= keep[0], x.y &= keep[1];
-                }
+            for (int n = 0; n < NT; ++n) {
+                const bool see = page && key >= st.lo[n] && key < st.hi[n];
+                if (!see) x[n][4 * j + i] = -__builtin_inff();
+                any |= see;
             }
+            if (any) keep[i / 2] |= i & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint4 &z = v.s[J > 1 ? j / 2 : 0][g];
+            if (J > 1 && (j & 1))
+                z.z &= keep[0], z.w &= keep[1];
+            else
+                z.x &= keep[0], z.y &= keep[1];
+        }
     }
+}
+
+/* Raises top and the bound of the V scales where a step passes them. */
+template <class F>
+__device__ __forceinline__ void check_step(State<F> &st, const float (&x)[F::NT][4 * F::J], const Half<F> &v) {
+    constexpr int NT = F::NT, G = F::G, J = F::J;
     float best[NT];
-    uint32_t dv[NT];
-    bool raise = false;
+    uint32_t dv = 0u;
+    bool raise  = false;
+#pragma unroll
+    for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < (J > 1 ? 4 : 2); ++i) dv = pk_max_u16(dv, word_of(v.s[b][g], i) & 0x7FFF7FFFu);
+    dv = max(dv & 0xFFFFu, dv >> 16);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        best[n] = sv[n][0];
-        dv[n]   = 0u;
+        best[n] = x[n][0];
 #pragma unroll
-        for (int i = 1; i < 4 * J; ++i) best[n] = fmaxf(best[n], sv[n][i]);
-#pragma unroll
-        for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int i = 0; i < (J > 1 ? 4 : 2); ++i)
-                    dv[n] = pk_max_u16(dv[n], word_of(vs[n][b][g], i) & 0x7FFF7FFFu);
-        dv[n] = max(dv[n] & 0xFFFFu, dv[n] >> 16);
-        raise |= best[n] > st.top[n] + kSlack || dv[n] > st.vmax[n];
+        for (int i = 1; i < 4 * J; ++i) best[n] = fmaxf(best[n], x[n][i]);
+        best[n] *= st.cs[n];
+        raise |= best[n] > st.top[n] + kSlack;
     }
+    raise |= dv > st.vmax;
     if (__any(raise)) {
+        dv      = max(dv, (uint32_t)__shfl_xor((int)dv, 16));
+        dv      = max(dv, (uint32_t)__shfl_xor((int)dv, 32));
+        st.vmax = max(dv, st.vmax);
+        /* a scale that is not finite gives NaN in its own dims alone */
+        const float z = (float)__builtin_bit_cast(_Float16, (uint16_t)min(st.vmax, 0x7BFFu));
+        const float e = (z > 0.0f ? (float)__builtin_amdgcn_frexp_expf(z) : 0.0f) - kLift;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             best[n] = fmaxf(best[n], __shfl_xor(best[n], 16));
             best[n] = fmaxf(best[n], __shfl_xor(best[n], 32));
-            dv[n]   = max(dv[n], (uint32_t)__shfl_xor((int)dv[n], 16));
-            dv[n]   = max(dv[n], (uint32_t)__shfl_xor((int)dv[n], 32));
-            st.vmax[n]    = max(dv[n], st.vmax[n]);
             st.top[n]     = fmaxf(st.top[n], best[n]);
-            /* a scale that is not finite gives NaN in its own dims alone */
-            const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)min(st.vmax[n], 0x7BFFu));
-            const float m = st.top[n] + (x > 0.0f ? (float)__builtin_amdgcn_frexp_expf(x) : 0.0f) - kLift;
+            const float m = st.top[n] + e;
             const float a = __builtin_amdgcn_exp2f(st.m[n] - m);
             st.l[n] *= a;
 #pragma unroll
@@ -339,33 +392,37 @@ __device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F
             st.m[n] = m;
         }
     }
+}
+
+/* p = exp2(cs x - m), O += codes . (p * scale) per block and group of dims. */
+template <class F>
+__device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F::J], const Half<F> &v,
+                                           uint32_t lane, const Magic &mg) {
+    constexpr int NT = F::NT, G = F::G, J = F::J, R = F::R;
+    const uint32_t u = (lane & 15u) / (16u / R);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4 * J; ++i) {
-            sv[n][i] = __builtin_amdgcn_exp2f(sv[n][i] - st.m[n]);
-            st.l[n] += sv[n][i];
+            x[n][i] = __builtin_amdgcn_exp2f(fmaf(x[n][i], st.cs[n], -st.m[n]));
+            st.l[n] += x[n][i];
         }
-    /* O += codes . (p * scale), per block and group of dims */
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         uint32_t ch[2], cl[2]; /* R > 1: this lane's 4 keys */
         if constexpr (R > 1) {
-            const uint4 z = vs[0][0][g];
+            const uint4 z = v.s[0][g];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t w = i ? z.y : z.x;
-                const float a = sv[0][2 * i] * half_lo(w), c = sv[0][2 * i + 1] * half_hi(w);
+                const float a = x[0][2 * i] * half_lo(w), c = x[0][2 * i + 1] * half_hi(w);
                 ch[i] = pk_rtz(a, c);
                 cl[i] = pk_rtz(a - half_lo(ch[i]), c - half_hi(ch[i]));
             }
         }
 #pragma unroll
         for (int b = 0; b < F::NB; ++b) {
-            union {
-                uint32_t u[4];
-                half8v v;
-            } wh[NT], wl[NT];
+            Words wh[NT], wl[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -375,15 +432,15 @@ __device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F
                         wh[n].u[i]      = mine ? ch[i & 1] : 0u;
                         wl[n].u[i]      = mine ? cl[i & 1] : 0u;
                     } else {
-                        const uint32_t w = word_of(vs[n][b][g], i);
-                        const float a = sv[n][8 * b + 2 * i] * half_lo(w), c = sv[n][8 * b + 2 * i + 1] * half_hi(w);
+                        const uint32_t w = word_of(v.s[b][g], i);
+                        const float a = x[n][8 * b + 2 * i] * half_lo(w), c = x[n][8 * b + 2 * i + 1] * half_hi(w);
                         wh[n].u[i] = pk_rtz(a, c);
                         wl[n].u[i] = pk_rtz(a - half_lo(wh[n].u[i]), c - half_hi(wh[n].u[i]));
                     }
                 }
 #pragma unroll
             for (int i = 2 * g; i < 2 * g + 2; ++i) {
-                const half8v a = unpack(word_of(d.v[b][i / 4], i & 3));
+                const half8v a = unpack_v(word_of(v.c[b][i / 4], i & 3), mg);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     st.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[n].v, st.o[n][i], 0, 0, 0);
@@ -394,32 +451,62 @@ __device__ __forceinline__ void run_step(State<F> &st, Step<F> &d, const Place<F
     }
 }
 
-/* Steps [a, b) of unit (s, ct, h): loads run one step ahead, table entries two. */
+/* Where a piece stands: the step whose P.V product comes next, and the places
+ * of it and of the two behind it. */
+struct Walk {
+    TableRow table;
+    uint32_t h, step, last; /* last: the piece's last step */
+    uint32_t in0, in1;      /* keys that every row of the tile attends */
+    Place at, next, after;
+};
+
+/* One step: its P.V product beside the S product of the next one, neither
+ * waiting for the other, while the loads of the next values and of the keys
+ * behind the next ones are under way. */
+template <class F>
+__device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk &w, float (&x)[F::NT][4 * F::J],
+                                          float (&y)[F::NT][4 * F::J], Half<F> &v, Half<F> &v_next,
+                                          const Half<F> &k_next, Half<F> &k_after, uint32_t lane, const Magic &mg) {
+    load_half<F, 1>(v_next, w.next, lane);
+    load_half<F, 0>(k_after, w.after, lane);
+    const Place coming  = place_of<F>(p.c, w.table, w.h, w.step + 3u < w.last ? w.step + 3u : w.last);
+    const uint32_t key0 = w.step * F::STEP;
+    if (!(key0 >= w.in0 && key0 + F::STEP <= w.in1 && w.at.there0 && w.at.there1))
+        mask_step<F>(x, v, st, w.at, key0, lane);
+    check_step<F>(st, x, v);
+    scores<F>(y, st, k_next, mg);
+    accumulate<F>(st, x, v, lane, mg);
+    w.at    = w.next;
+    w.next  = w.after;
+    w.after = coming;
+}
+
+/* Steps [a, b) of unit (s, ct, h). */
 template <class F>
 __device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t h,
                                           const lfm_q4_tile &t, uint32_t pos0, uint32_t a, uint32_t b, uint32_t lane) {
-    const int32_t *table = p.c.table + (size_t)s * p.c.table_stride;
-    /* keys that every row of the tile attends */
-    const uint32_t in0 = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window), in1 = pos0 + t.r0 + 1u;
-    Place<F> at = place_of<F>(p.c, table, h, a);
-    Step<F> d;
-    load_step<F>(d, at, lane);
-    Place<F> next = place_of<F>(p.c, table, h, a + 1u < b ? a + 1u : a);
-    for (uint32_t step = a; step < b; ++step) {
-        Step<F> e;
-        load_step<F>(e, next, lane);
-        const Place<F> after = place_of<F>(p.c, table, h, step + 2u < b ? step + 2u : b - 1u);
-        const uint32_t key0  = step * F::STEP;
-        bool inner           = key0 >= in0 && key0 + F::STEP <= in1;
-#pragma unroll
-        for (int i = 0; i < F::NB; ++i) inner = inner && at.there[i];
-        if (inner)
-            run_step<F, false>(st, d, at, key0, lane);
-        else
-            run_step<F, true>(st, d, at, key0, lane);
-        d    = e;
-        at   = next;
-        next = after;
+    const Magic mg = magic();
+    Walk w;
+    w.table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
+    w.h     = h;
+    w.step  = a;
+    w.last  = b - 1u;
+    w.in0   = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window);
+    w.in1   = pos0 + t.r0 + 1u;
+    w.at    = place_of<F>(p.c, w.table, h, a);
+    w.next  = place_of<F>(p.c, w.table, h, a < w.last ? a + 1u : w.last);
+    w.after = place_of<F>(p.c, w.table, h, a + 2u < w.last ? a + 2u : w.last);
+    Half<F> k0, k1, v0, v1;
+    load_half<F, 0>(k0, w.at, lane);
+    load_half<F, 1>(v0, w.at, lane);
+    load_half<F, 0>(k1, w.next, lane);
+    float x[F::NT][4 * F::J], y[F::NT][4 * F::J];
+    scores<F>(x, st, k0, mg);
+    for (;;) { /* buffers change roles every step: two steps per turn, no copies */
+        step_once<F>(st, p, w, x, y, v0, v1, k1, k0, lane, mg);
+        if (++w.step == b) break;
+        step_once<F>(st, p, w, y, x, v1, v0, k0, k1, lane, mg);
+        if (++w.step == b) break;
     }
 }
 
@@ -537,10 +624,8 @@ template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(c
     uint32_t total = 0u;
     for (uint32_t e0 = 0; e0 < n_e; e0 += 64u) {
         const uint32_t inc = wave_scan(entry_steps(p, e0 + lane, n_e), lane);
-        if (wave == 0u && e0 + lane < n_e) p.pre[e0 + lane + 1u] = total + inc;
         total += uniform((uint32_t)__shfl((int)inc, 63));
     }
-    if (wave == 0u && lane == 0u) p.pre[0] = 0u;
     const uint64_t N = (uint64_t)total * nh;
     if (N == 0u) return;
     const uint32_t G = lfm_q4_waves(&p.plan, N);
@@ -576,10 +661,13 @@ template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(c
             start<F>(st, p, s, ct, h, pos0, rows, lane);
             run_piece<F>(st, p, s, h, tile, pos0, tile.step0 + a, tile.step0 + b, lane);
             join_lanes<F>(st);
+            const uint32_t unit = e * nh + h;
+            if (lane == 0u && a == 0u) p.range[unit].x = wave;
+            if (lane == 0u && b == tile.n_steps) p.range[unit].y = wave;
             if (a == 0u && b == tile.n_steps)
                 write_out<F>(st, p, s, ct, h, rows, lane);
             else
-                write_part<F>(st, p, (uint64_t)wave + (uint64_t)e * nh + h, lane);
+                write_part<F>(st, p, (uint64_t)wave + unit, lane);
             t = te;
         }
         before += tile.n_steps;
@@ -588,30 +676,26 @@ template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(c
 }
 
 /* The pieces of every unit that more than one wave holds: one workgroup per
- * (unit, column); HD / 4 threads take a piece, 1024 / HD pieces at a time. */
-template <int HD> __global__ __launch_bounds__(256) void k_paged_merge(const GqaParams p) {
-    constexpr uint32_t L = HD / 4, P = 256u / L;
+ * (unit, column); HD / 4 threads take a piece, T / (HD / 4) pieces at a time. */
+template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(const GqaParams p) {
+    constexpr uint32_t L = HD / 4, P = T / L;
     __shared__ float sm[P], sl[P];
     __shared__ float4 so[P][L];
     const uint32_t nh = p.c.n_head_kv, cols = p.plan.cols;
     const uint32_t unit = blockIdx.x / cols, col = blockIdx.x - unit * cols;
     const uint32_t e = unit / nh, h = unit - e * nh;
-    const uint32_t n = p.pre[e + 1u] - p.pre[e];
-    if (n == 0u) return;
-    const uint64_t N = (uint64_t)p.pre[p.c.n_seq * p.plan.n_ct] * nh, first = (uint64_t)p.pre[e] * nh + (uint64_t)h * n;
-    const uint32_t G = lfm_q4_waves(&p.plan, N);
-    const uint32_t g0 = lfm_q4_owner(first, N, G), g1 = lfm_q4_owner(first + n - 1u, N, G);
-    if (g0 == g1) return;
     const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
+    const uint2 g       = p.range[unit]; /* not written, and not used, where the column has no row */
     const uint32_t rows = rows_of(p.c, s, p.c.pos0[s]);
     const uint32_t mul = p.plan.kv_mul, ci = ct * cols + col, row = ci / mul;
-    if (row >= rows) return;
+    if (row >= rows || g.x == g.y) return;
+    const uint32_t g0 = g.x, g1 = g.y;
     const size_t head = ((size_t)s * p.c.n_rows + row) * (nh * mul) + h * mul + (ci - row * mul);
     const uint32_t i = threadIdx.x % L, k = threadIdx.x / L;
     float m = kNoScore, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t g = g0 + k; g <= g1; g += P) {
-        const size_t at = ((size_t)g + unit) * cols + col;
+    for (uint32_t w = g0 + k; w <= g1; w += P) {
+        const size_t at = ((size_t)w + unit) * cols + col;
         const float2 ml = p.part_ml[at];
         const float4 x  = reinterpret_cast<const float4 *>(p.part_o + at * HD)[i];
         const float mn = fmaxf(m, ml.x), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(ml.x - mn);
@@ -646,7 +730,7 @@ struct Launch {
     lfm_q4_plan plan;
     uint32_t copies, tiles; /* R and NT of the form */
     bool split;
-    size_t o_bytes, ml_bytes, pre_bytes;
+    size_t o_bytes, ml_bytes, range_bytes;
 };
 
 int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q, uint32_t n_head_kv,
@@ -682,7 +766,7 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     const uint64_t slots = L->split ? p.n_waves + units : 0u;
     L->o_bytes   = slots * p.cols * head_dim * 4u;
     L->ml_bytes  = slots * p.cols * 8u;
-    L->pre_bytes = L->split ? (entries + 1u) * 4u : 0u;
+    L->range_bytes = L->split ? units * 8u : 0u;
     return LFM_ATTN_OK;
 }
 
@@ -690,7 +774,13 @@ template <class F> void launch_form(const GqaParams &p, bool split, hipStream_t 
     const uint64_t units = (uint64_t)p.c.n_seq * p.plan.n_ct * p.c.n_head_kv;
     if (split) {
         hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
-        hipLaunchKernelGGL(k_paged_merge<F::HD>, dim3((uint32_t)(units * p.plan.cols)), dim3(256), 0, stream, p);
+        /* a wave per column where the units alone nearly fill the card: few pieces each */
+        if (units * 8u >= kWaves)
+            hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3((uint32_t)(units * p.plan.cols)), dim3(64), 0, stream,
+                               p);
+        else
+            hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3((uint32_t)(units * p.plan.cols)), dim3(512), 0, stream,
+                               p);
     } else {
         hipLaunchKernelGGL(k_paged_gqa<F>, dim3((uint32_t)((units + 3u) / 4u)), dim3(256), 0, stream, p);
     }
@@ -703,7 +793,7 @@ int paged_q4_gqa_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     Launch L;
     const int st = plan_launch(&L, n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, capacity, window);
     if (st != LFM_ATTN_OK) return st;
-    *bytes = L.o_bytes + L.ml_bytes + L.pre_bytes;
+    *bytes = L.o_bytes + L.ml_bytes + L.range_bytes;
     return LFM_ATTN_OK;
 }
 
@@ -725,7 +815,7 @@ int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int
     uint8_t *w      = static_cast<uint8_t *>(workspace);
     p.part_o        = reinterpret_cast<float *>(w);
     p.part_ml       = reinterpret_cast<float2 *>(w + L.o_bytes);
-    p.pre           = reinterpret_cast<uint32_t *>(w + L.o_bytes + L.ml_bytes);
+    p.range         = reinterpret_cast<uint2 *>(w + L.o_bytes + L.ml_bytes);
     if (c.head_dim == 64u) {
         if (L.copies == 4u)
             launch_form<Form<64, 1, 4, 2>>(p, L.split, stream);
