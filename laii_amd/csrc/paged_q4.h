@@ -54,20 +54,21 @@ LFM_IDX_FN uint32_t lfm_q4_scale(uint32_t head_dim, uint32_t v, uint32_t t, uint
 /* ---- attention: units, steps, shares -------------------------------------------
  * The query columns of a (sequence, KV head) are its rows x kv_mul query heads,
  * row major, cut into tiles of `cols`.  A unit is (sequence, tile, KV head),
- * numbered in that order; its work is the steps of `step` keys that cover the
- * keys its rows attend.  Wave g of G takes steps [g N / G, (g + 1) N / G) of the
- * batch's N, cut at units; the piece of wave g in unit v has partial slot
- * g + v: along the walk g or v grows, so slots are unique and below G + units.
- * A unit that one wave covers whole is written directly. */
+ * numbered in that order; its work is the steps of 2^step_shift keys that cover
+ * the keys its rows attend.  The batch's N < 2^32 steps, in unit order, go to G
+ * waves in equal shares (the first N % G one longer), cut at units; the piece of
+ * wave g in unit v has partial slot g + v: along the walk g or v grows, so slots
+ * are unique and below G + units.  A unit that one wave covers whole is written
+ * directly.  Everything here is 32-bit: a 64-bit division costs a wave more than
+ * a step of keys. */
 typedef struct {
     uint32_t n_seq, n_rows, kv_mul, n_head_kv;
-    uint32_t window;    /* 0: none                                    */
-    uint32_t capacity;  /* positions a sequence's table reaches, <= 2^31 */
-    uint32_t cols;      /* query columns per tile                     */
-    uint32_t step;      /* keys per step, a multiple of 32            */
-    uint32_t n_ct;      /* tiles per sequence                         */
-    uint32_t min_steps; /* fewest steps per wave                      */
-    uint32_t n_waves;   /* waves launched                             */
+    uint32_t window;     /* 0: none                                      */
+    uint32_t capacity;   /* positions a sequence's table reaches, <= 2^31 */
+    uint32_t cols;       /* query columns per tile                       */
+    uint32_t step_shift; /* log2 of the keys per step, at least 5        */
+    uint32_t n_ct;       /* tiles per sequence                           */
+    uint32_t n_waves;    /* waves launched                               */
 } lfm_q4_plan;
 
 /* Rows of a sequence that count: of its n_rows_seq (or all n_rows) those whose
@@ -81,8 +82,7 @@ LFM_IDX_FN uint32_t lfm_q4_rows(uint32_t pos0, uint32_t rows, uint32_t n_rows, u
 /* Rows and steps of tile ct of a sequence whose `rows` rows that count start
  * at position pos0.  n_steps 0: the tile has no rows. */
 typedef struct {
-    uint32_t r0, r1;        /* rows [r0, r1)                          */
-    uint32_t lo, hi;        /* keys [lo, hi) of all its rows           */
+    uint32_t r0, r1; /* rows [r0, r1) */
     uint32_t step0, n_steps;
 } lfm_q4_tile;
 
@@ -92,31 +92,32 @@ LFM_IDX_FN uint32_t lfm_q4_row_lo(uint32_t pos, uint32_t window) {
 
 LFM_IDX_FN lfm_q4_tile lfm_q4_tile_of(const lfm_q4_plan *p, uint32_t pos0, uint32_t rows, uint32_t ct) {
     lfm_q4_tile t;
-    const uint32_t cols = rows * p->kv_mul, c0 = ct * p->cols;
-    t.r0 = t.r1 = t.lo = t.hi = t.step0 = t.n_steps = 0u;
-    if (c0 >= cols) return t;
-    const uint32_t c1 = cols - c0 < p->cols ? cols : c0 + p->cols;
-    t.r0              = c0 / p->kv_mul;
-    t.r1              = (c1 - 1u) / p->kv_mul + 1u;
-    t.lo              = lfm_q4_row_lo(pos0 + t.r0, p->window);
-    t.hi              = pos0 + t.r1;
-    t.step0           = t.lo / p->step;
-    t.n_steps         = (t.hi + p->step - 1u) / p->step - t.step0;
+    t.r0 = t.r1 = t.step0 = t.n_steps = 0u;
+    if (p->n_ct == 1u) { /* one tile holds every row */
+        t.r1 = rows;
+    } else {
+        const uint32_t cols = rows * p->kv_mul, c0 = ct * p->cols;
+        if (c0 >= cols) return t;
+        const uint32_t c1 = cols - c0 < p->cols ? cols : c0 + p->cols;
+        t.r0              = c0 / p->kv_mul;
+        t.r1              = (c1 - 1u) / p->kv_mul + 1u;
+    }
+    if (t.r1 == 0u) return t;
+    t.step0   = lfm_q4_row_lo(pos0 + t.r0, p->window) >> p->step_shift;
+    t.n_steps = ((pos0 + t.r1 - 1u) >> p->step_shift) + 1u - t.step0;
     return t;
 }
 
 /* Waves taking part, for N steps in all. */
-LFM_IDX_FN uint32_t lfm_q4_waves(const lfm_q4_plan *p, uint64_t n_steps) {
-    uint64_t g = n_steps / p->min_steps;
-    if (g > p->n_waves) g = p->n_waves;
-    return (uint32_t)(g ? g : 1u);
+LFM_IDX_FN uint32_t lfm_q4_waves(const lfm_q4_plan *p, uint32_t n_steps) {
+    return n_steps < p->n_waves ? n_steps : p->n_waves;
 }
 
-LFM_IDX_FN uint64_t lfm_q4_share(uint32_t wave, uint64_t n_steps, uint32_t G) { return (uint64_t)wave * n_steps / G; }
-
-/* Wave holding step t of N. */
-LFM_IDX_FN uint32_t lfm_q4_owner(uint64_t t, uint64_t n_steps, uint32_t G) {
-    return (uint32_t)(((t + 1u) * G - 1u) / n_steps);
+/* Steps [*t0, *t1) of wave g < G. */
+LFM_IDX_FN void lfm_q4_share(uint32_t g, uint32_t n_steps, uint32_t G, uint32_t *t0, uint32_t *t1) {
+    const uint32_t q = n_steps / G, r = n_steps - q * G;
+    *t0 = g * q + (g < r ? g : r);
+    *t1 = *t0 + q + (g < r ? 1u : 0u);
 }
 
 #endif

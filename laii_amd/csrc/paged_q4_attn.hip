@@ -103,12 +103,20 @@ __device__ __forceinline__ half8v unpack_k(uint32_t w, const Magic &k) {
     return r.v;
 }
 
-__device__ __forceinline__ uint32_t pk_rtz(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-}
-
 __device__ __forceinline__ float half_lo(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[0]; }
 __device__ __forceinline__ float half_hi(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[1]; }
+
+/* Two weights p * d as fp16 hi + lo: hi is the product rounded, lo what is
+ * left of it, rounded; one mixed-precision fma each. */
+__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t d, uint32_t *hi, uint32_t *lo) {
+    half2v h, l;
+    h[0] = (_Float16)fmaf(p0, half_lo(d), 0.0f);
+    h[1] = (_Float16)fmaf(p1, half_hi(d), 0.0f);
+    l[0] = (_Float16)fmaf(p0, half_lo(d), -(float)h[0]);
+    l[1] = (_Float16)fmaf(p1, half_hi(d), -(float)h[1]);
+    *hi  = __builtin_bit_cast(uint32_t, h);
+    *lo  = __builtin_bit_cast(uint32_t, l);
+}
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -119,9 +127,10 @@ __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
  * takes every R-th 16-key tile of a step: softmax work shrinks by R.  The query
  * operand is kept R times, zero outside copy r's columns, so that the S product of
  * tile t with copy t % R leaves each column the tile that it takes, with no
- * selection.  NB: blocks of 32 keys per step. */
-template <int HD_, int NT_, int R_, int NB_> struct Form {
-    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_;
+ * selection.  NB: blocks of 32 keys per step.  OCC: waves per SIMD that the
+ * registers are cut for. */
+template <int HD_, int NT_, int R_, int NB_, int OCC_> struct Form {
+    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_, OCC = OCC_;
     static constexpr int G = HD / 32, DT = HD / 16, TILES = 2 * NB, J = TILES / R;
     static constexpr int COLS = R > 1 ? 16 / R : 16 * NT, STEP = 32 * NB;
     static_assert(R == 1 || (NT == 1 && J == 1), "a copy takes one tile per step");
@@ -235,19 +244,26 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
         big = fmaxf(big, __shfl_xor(big, 16));
         big = fmaxf(big, __shfl_xor(big, 32));
         const int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
+        const float unit = ldexpf(p.scale < 0.0f ? -1.0f : 1.0f, -e);
 #pragma unroll
         for (int g = 0; g < F::G; ++g) {
             float sum = 0.0f;
+            Words yh, yl;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y     = ldexpf(p.scale < 0.0f ? -x[g][i] : x[g][i], -e);
-                const _Float16 yh = (_Float16)y, yl = (_Float16)(y - (float)yh);
-                if (i & 2) sum += (float)yh + (float)yl;
+                const float y = x[g][i] * unit;
+                yh.v[i]       = (_Float16)y;
+                yl.v[i]       = (_Float16)(y - (float)yh.v[i]);
+                if (i & 2) sum += (float)yh.v[i] + (float)yl.v[i];
+            }
 #pragma unroll
-                for (int r = 0; r < F::R; ++r) {
-                    st.qh[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yh : (_Float16)0.0f;
-                    st.ql[n][r][g][i] = F::R == 1 || u == (uint32_t)r ? yl : (_Float16)0.0f;
-                }
+            for (int r = 0; r < F::R; ++r) {
+                const uint32_t mine = F::R == 1 || u == (uint32_t)r ? 0xFFFFFFFFu : 0u;
+                Words a, z;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a.u[i] = yh.u[i] & mine, z.u[i] = yl.u[i] & mine;
+                st.qh[n][r][g] = a.v;
+                st.ql[n][r][g] = z.v;
             }
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
@@ -413,12 +429,8 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
         if constexpr (R > 1) {
             const uint4 z = v.s[0][g];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t w = i ? z.y : z.x;
-                const float a = x[0][2 * i] * half_lo(w), c = x[0][2 * i + 1] * half_hi(w);
-                ch[i] = pk_rtz(a, c);
-                cl[i] = pk_rtz(a - half_lo(ch[i]), c - half_hi(ch[i]));
-            }
+            for (int i = 0; i < 2; ++i)
+                split_weights(x[0][2 * i], x[0][2 * i + 1], i ? z.y : z.x, &ch[i], &cl[i]);
         }
 #pragma unroll
         for (int b = 0; b < F::NB; ++b) {
@@ -432,10 +444,8 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
                         wh[n].u[i]      = mine ? ch[i & 1] : 0u;
                         wl[n].u[i]      = mine ? cl[i & 1] : 0u;
                     } else {
-                        const uint32_t w = word_of(v.s[b][g], i);
-                        const float a = x[n][8 * b + 2 * i] * half_lo(w), c = x[n][8 * b + 2 * i + 1] * half_hi(w);
-                        wh[n].u[i] = pk_rtz(a, c);
-                        wl[n].u[i] = pk_rtz(a - half_lo(wh[n].u[i]), c - half_hi(wh[n].u[i]));
+                        split_weights(x[n][8 * b + 2 * i], x[n][8 * b + 2 * i + 1], word_of(v.s[b][g], i),
+                                      &wh[n].u[i], &wl[n].u[i]);
                     }
                 }
 #pragma unroll
@@ -481,10 +491,12 @@ __device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk
     w.after = coming;
 }
 
-/* Steps [a, b) of unit (s, ct, h). */
+/* Steps [a, b) of unit (s, ct, h) into a fresh state.  The first loads go out
+ * before the queries are read and split. */
 template <class F>
-__device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t h,
-                                          const lfm_q4_tile &t, uint32_t pos0, uint32_t a, uint32_t b, uint32_t lane) {
+__device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
+                                          const lfm_q4_tile &t, uint32_t pos0, uint32_t rows, uint32_t a, uint32_t b,
+                                          uint32_t lane) {
     const Magic mg = magic();
     Walk w;
     w.table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
@@ -500,6 +512,7 @@ __device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint
     load_half<F, 0>(k0, w.at, lane);
     load_half<F, 1>(v0, w.at, lane);
     load_half<F, 0>(k1, w.next, lane);
+    start<F>(st, p, s, ct, h, pos0, rows, lane);
     float x[F::NT][4 * F::J], y[F::NT][4 * F::J];
     scores<F>(x, st, k0, mg);
     for (;;) { /* buffers change roles every step: two steps per turn, no copies */
@@ -564,17 +577,18 @@ __device__ __forceinline__ void write_out(const State<F> &st, const GqaParams &p
     }
 }
 
+/* A piece's columns as they stand: outputs [col][HD], (m, l) [col]. */
 template <class F>
-__device__ __forceinline__ void write_part(const State<F> &st, const GqaParams &p, uint64_t slot, uint32_t lane) {
+__device__ __forceinline__ void put_part(const State<F> &st, float *o, float2 *ml, uint32_t lane) {
     const uint32_t col = lane & 15u, kg = lane >> 4;
 #pragma unroll
     for (int n = 0; n < F::NT; ++n) {
         if (F::R > 1 && col >= 16u / F::R) continue;
-        const size_t at = (size_t)slot * F::COLS + n * 16u + col;
-        if (kg == 0u) p.part_ml[at] = make_float2(st.m[n], st.l[n]);
+        const uint32_t c = n * 16u + col;
+        if (kg == 0u) ml[c] = make_float2(st.m[n], st.l[n]);
 #pragma unroll
         for (int i = 0; i < F::DT; ++i)
-            reinterpret_cast<float4 *>(p.part_o + at * F::HD)[i * 4 + kg] =
+            reinterpret_cast<float4 *>(o + c * F::HD)[i * 4 + kg] =
                 make_float4(st.o[n][i][0], st.o[n][i][1], st.o[n][i][2], st.o[n][i][3]);
     }
 }
@@ -583,28 +597,80 @@ __device__ __forceinline__ uint32_t rows_of(const PagedQ4 &c, uint32_t s, uint32
     return lfm_q4_rows(pos0, c.rows_seq ? c.rows_seq[s] : c.n_rows, c.n_rows, c.capacity);
 }
 
-/* Every wave one unit, all its keys. */
-template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa(const GqaParams p) {
+/* Every wave one unit, all its keys: 4 adjacent tiles of a (sequence, KV head)
+ * per workgroup, which read the same pages at about the same time.  The last
+ * tiles, with the most keys, are dispatched first; consecutive workgroups, which
+ * go to the 8 XCDs in turn, differ in KV head, so a head's pages mostly stay in
+ * one XCD's L2. */
+template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa(const GqaParams p) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t unit = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
-    const uint32_t h = unit % p.c.n_head_kv, sc = unit / p.c.n_head_kv;
-    const uint32_t s = sc / p.plan.n_ct, ct = sc - s * p.plan.n_ct;
-    if (s >= p.c.n_seq) return;
+    const uint32_t pairs = p.c.n_seq * p.c.n_head_kv, quad = blockIdx.x / pairs, pair = blockIdx.x - quad * pairs;
+    const uint32_t s = pair / p.c.n_head_kv, h = pair - s * p.c.n_head_kv;
+    const uint32_t back = quad * 4u + uniform(threadIdx.x >> 6);
+    if (back >= p.plan.n_ct) return;
+    const uint32_t ct   = p.plan.n_ct - 1u - back;
     const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
     const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
     if (t.n_steps == 0u) return;
     State<F> st;
-    start<F>(st, p, s, ct, h, pos0, rows, lane);
-    run_piece<F>(st, p, s, h, t, pos0, t.step0, t.step0 + t.n_steps, lane);
+    run_piece<F>(st, p, s, ct, h, t, pos0, rows, t.step0, t.step0 + t.n_steps, lane);
     join_lanes<F>(st);
     write_out<F>(st, p, s, ct, h, rows, lane);
 }
 
-/* Steps of entry e (sequence, tile), 0 past the last. */
-__device__ __forceinline__ uint32_t entry_steps(const GqaParams &p, uint32_t e, uint32_t n_entries) {
-    if (e >= n_entries) return 0u;
-    const uint32_t s = e / p.plan.n_ct, pos0 = p.c.pos0[s];
-    return lfm_q4_tile_of(&p.plan, pos0, rows_of(p.c, s, pos0), e - s * p.plan.n_ct).n_steps;
+/* One workgroup of W waves per unit: its waves share the steps and join in
+ * LDS.  For short units: one launch, no partials. */
+template <class F, int W> __global__ __launch_bounds__(64 * W, 2) void k_paged_gqa_wg(const GqaParams p) {
+    __shared__ __align__(16) float so[W][F::COLS][F::HD];
+    __shared__ float2 sml[W][F::COLS];
+    const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6);
+    const uint32_t unit = blockIdx.x, h = unit % p.c.n_head_kv, sc = unit / p.c.n_head_kv;
+    const uint32_t s = sc / p.plan.n_ct, ct = sc - s * p.plan.n_ct;
+    const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
+    const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
+    if (t.n_steps == 0u) return;
+    uint32_t a, b;
+    lfm_q4_share(wave, t.n_steps, W, &a, &b);
+    const uint32_t parts = t.n_steps < W ? t.n_steps : W; /* the first shares are the longer ones */
+    a = uniform(a), b = uniform(b);
+    if (a < b) {
+        State<F> st;
+        run_piece<F>(st, p, s, ct, h, t, pos0, rows, t.step0 + a, t.step0 + b, lane);
+        join_lanes<F>(st);
+        put_part<F>(st, &so[wave][0][0], &sml[wave][0], lane);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < F::COLS * F::HD / 4u; i += 64u * W) {
+        const uint32_t col = i / (F::HD / 4u), d = i % (F::HD / 4u);
+        const size_t head  = head_of<F>(p, s, h, rows, ct * F::COLS + col);
+        if (head == ~(size_t)0) continue;
+        float m = kNoScore, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t w = 0; w < parts; ++w) m = fmaxf(m, sml[w][col].x);
+        for (uint32_t w = 0; w < parts; ++w) {
+            const float2 ml = sml[w][col];
+            const float f   = __builtin_amdgcn_exp2f(ml.x - m);
+            const float4 x  = reinterpret_cast<const float4 *>(so[w][col])[d];
+            l += ml.y * f;
+            o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+        }
+        const float f = out_factor(p, l, head);
+        reinterpret_cast<float4 *>(p.out + head * F::HD)[d] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    }
+}
+
+/* Position, rows and steps of entry e (sequence, tile); no steps past the last. */
+struct Entry {
+    uint32_t pos0, rows, steps;
+};
+__device__ __forceinline__ Entry entry_of(const GqaParams &p, uint32_t e, uint32_t n_entries) {
+    Entry r = {0u, 0u, 0u};
+    if (e >= n_entries) return r;
+    const uint32_t s = p.plan.n_ct == 1u ? e : e / p.plan.n_ct;
+    r.pos0           = p.c.pos0[s];
+    r.rows           = rows_of(p.c, s, r.pos0);
+    r.steps          = lfm_q4_tile_of(&p.plan, r.pos0, r.rows, e - s * p.plan.n_ct).n_steps;
+    return r;
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t lane) { /* inclusive */
@@ -616,62 +682,61 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t lane) { /* in
     return x;
 }
 
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t i) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)i);
+}
+
 /* Equal shares of the batch's steps per wave. */
-template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(const GqaParams p) {
+template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa_split(const GqaParams p) {
     const uint32_t lane = threadIdx.x & 63u, nh = p.c.n_head_kv;
     const uint32_t wave = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
     const uint32_t n_e  = p.c.n_seq * p.plan.n_ct;
-    uint32_t total = 0u;
-    for (uint32_t e0 = 0; e0 < n_e; e0 += 64u) {
-        const uint32_t inc = wave_scan(entry_steps(p, e0 + lane, n_e), lane);
-        total += uniform((uint32_t)__shfl((int)inc, 63));
-    }
-    const uint64_t N = (uint64_t)total * nh;
-    if (N == 0u) return;
-    const uint32_t G = lfm_q4_waves(&p.plan, N);
+    /* a window of 64 entries, one per lane; batches of up to 64 keep it */
+    Entry en        = entry_of(p, lane, n_e);
+    uint32_t inc    = wave_scan(en.steps, lane);
+    uint32_t total  = lane_of(inc, 63u);
+    for (uint32_t e0 = 64u; e0 < n_e; e0 += 64u)
+        total += lane_of(wave_scan(entry_of(p, e0 + lane, n_e).steps, lane), 63u);
+    const uint32_t N = total * nh, G = lfm_q4_waves(&p.plan, N);
     if (wave >= G) return;
-    uint64_t t        = lfm_q4_share(wave, N, G);
-    const uint64_t t1 = lfm_q4_share(wave + 1u, N, G);
-    /* the entry holding step t */
-    uint32_t e = 0u, before = 0u, want = (uint32_t)(t / nh);
-    for (uint32_t e0 = 0;; e0 += 64u) {
-        const uint32_t n = entry_steps(p, e0 + lane, n_e), inc = wave_scan(n, lane);
-        const uint64_t hit = __ballot(before + inc > want);
-        if (hit) {
-            const int i = __builtin_ctzll(hit);
-            e           = e0 + (uint32_t)i;
-            before += uniform((uint32_t)__shfl((int)(inc - n), i));
-            break;
-        }
-        before += uniform((uint32_t)__shfl((int)inc, 63));
-    }
-    e = uniform(e);
+    uint32_t t, t1;
+    lfm_q4_share(wave, N, G, &t, &t1);
+    t  = uniform(t);
+    t1 = uniform(t1);
+    uint32_t e0 = 0u, base = 0u; /* the window's first entry, steps before it */
     while (t < t1) {
-        const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
-        const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
-        const lfm_q4_tile tile = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
-        const uint64_t first   = (uint64_t)before * nh;
-        while (t < t1 && t < first + (uint64_t)tile.n_steps * nh) {
-            const uint32_t h  = uniform((uint32_t)((t - first) / tile.n_steps));
-            const uint64_t u0 = first + (uint64_t)h * tile.n_steps;
-            const uint64_t u1 = u0 + tile.n_steps;
-            const uint64_t te = t1 < u1 ? t1 : u1;
-            const uint32_t a = uniform((uint32_t)(t - u0)), b = uniform((uint32_t)(te - u0));
-            State<F> st;
-            start<F>(st, p, s, ct, h, pos0, rows, lane);
-            run_piece<F>(st, p, s, h, tile, pos0, tile.step0 + a, tile.step0 + b, lane);
-            join_lanes<F>(st);
-            const uint32_t unit = e * nh + h;
-            if (lane == 0u && a == 0u) p.range[unit].x = wave;
-            if (lane == 0u && b == tile.n_steps) p.range[unit].y = wave;
-            if (a == 0u && b == tile.n_steps)
-                write_out<F>(st, p, s, ct, h, rows, lane);
-            else
-                write_part<F>(st, p, (uint64_t)wave + unit, lane);
-            t = te;
+        const uint32_t want = uniform(t / nh);
+        uint64_t hit        = __ballot(base + inc > want);
+        while (!hit) { /* ends: want is below the total */
+            base += lane_of(inc, 63u);
+            e0 += 64u;
+            en  = entry_of(p, e0 + lane, n_e);
+            inc = wave_scan(en.steps, lane);
+            hit = __ballot(base + inc > want);
         }
-        before += tile.n_steps;
-        ++e;
+        const uint32_t i = (uint32_t)__builtin_ctzll(hit), e = e0 + i;
+        const uint32_t pos0 = lane_of(en.pos0, i), rows = lane_of(en.rows, i), n = lane_of(en.steps, i);
+        const uint32_t first = (base + lane_of(inc, i) - n) * nh;
+        const uint32_t s = p.plan.n_ct == 1u ? e : uniform(e / p.plan.n_ct), ct = e - s * p.plan.n_ct;
+        const lfm_q4_tile tile = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
+        uint32_t h = uniform((t - first) / n);
+        uint32_t a = t - first - h * n;
+        for (; t < t1 && h < nh; ++h, a = 0u) {
+            const uint32_t b    = n - a < t1 - t ? n : a + (t1 - t);
+            const uint32_t unit = e * nh + h;
+            State<F> st;
+            run_piece<F>(st, p, s, ct, h, tile, pos0, rows, tile.step0 + a, tile.step0 + b, lane);
+            join_lanes<F>(st);
+            if (lane == 0u && a == 0u) p.range[unit].x = wave;
+            if (lane == 0u && b == n) p.range[unit].y = wave;
+            if (a == 0u && b == n) {
+                write_out<F>(st, p, s, ct, h, rows, lane);
+            } else {
+                const size_t at = ((size_t)wave + unit) * F::COLS;
+                put_part<F>(st, p.part_o + at * F::HD, p.part_ml + at, lane);
+            }
+            t += b - a;
+        }
     }
 }
 
@@ -724,12 +789,13 @@ template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(cons
 }
 
 /* ---- host: forms, split, scratch ------------------------------------------------ */
-constexpr uint32_t kWaves = 2048u; /* two per SIMD of 256 compute units */
+constexpr uint32_t kCus        = 256u;
+constexpr uint32_t kGroupSteps = 24u;
 
 struct Launch {
     lfm_q4_plan plan;
-    uint32_t copies, tiles; /* R and NT of the form */
-    bool split;
+    uint32_t copies, tiles, occ; /* R, NT and OCC of the form */
+    enum { kDirect, kSplit, kGroup } how;
     size_t o_bytes, ml_bytes, range_bytes;
 };
 
@@ -747,43 +813,55 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     p.capacity  = capacity;
     L->tiles    = 1u;
     L->copies   = 1u;
-    if (head_dim == 64u && cols <= 4u) L->copies = 4u;
-    if (head_dim == 128u && cols <= 8u) L->copies = 2u;
+    L->occ      = 2u;
+    if (head_dim == 64u) {
+        if (cols <= 4u) L->copies = 4u;
+        if (cols > 16u) L->tiles = 2u;
+    } else {
+        if (cols <= 8u) L->copies = 2u;
+        if (cols > 8u) L->occ = 1u;
+        if (cols > 16u) L->tiles = 2u;
+    }
     p.cols = L->copies > 1u ? 16u / L->copies : 16u * L->tiles;
-    p.step = L->copies == 4u ? 64u : 32u;
+    p.step_shift = L->copies == 4u ? 6u : 5u;
     p.n_ct = (uint32_t)((cols + p.cols - 1u) / p.cols);
-    p.min_steps = 1u;
     const uint64_t entries = (uint64_t)n_seq * p.n_ct, units = entries * n_head_kv;
     if (units > 0x7FFFFFFFull / p.cols) return LFM_ATTN_E_UNSUPPORTED;
     uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
     if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
-    const uint64_t steps = (keys + p.step - 1u) / p.step + (window ? 1u : 0u);
+    const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u);
+    const uint32_t resident = 4u * kCus * L->occ; /* waves */
     /* enough units fill the card by themselves; step counts of a split are 32 bits */
-    L->split = units < 2u * kWaves && entries * (capacity / 32u) < 0xFFFFFFFFull;
-    uint64_t waves = units * steps / p.min_steps;
-    if (waves > kWaves) waves = kWaves;
+    L->how = units < 2u * resident && units * (capacity / 32u) < 0x80000000ull ? Launch::kSplit : Launch::kDirect;
+    if (units <= 512u && steps <= kGroupSteps && L->occ == 2u) L->how = Launch::kGroup;
+    uint64_t waves = units * steps;
+    if (waves > resident) waves = resident;
     p.n_waves    = (uint32_t)((waves + 3u) / 4u * 4u);
-    const uint64_t slots = L->split ? p.n_waves + units : 0u;
-    L->o_bytes   = slots * p.cols * head_dim * 4u;
-    L->ml_bytes  = slots * p.cols * 8u;
-    L->range_bytes = L->split ? units * 8u : 0u;
+    const uint64_t slots = L->how == Launch::kSplit ? p.n_waves + units : 0u;
+    L->o_bytes     = slots * p.cols * head_dim * 4u;
+    L->ml_bytes    = slots * p.cols * 8u;
+    L->range_bytes = L->how == Launch::kSplit ? units * 8u : 0u;
     return LFM_ATTN_OK;
 }
 
-template <class F> void launch_form(const GqaParams &p, bool split, hipStream_t stream) {
-    const uint64_t units = (uint64_t)p.c.n_seq * p.plan.n_ct * p.c.n_head_kv;
-    if (split) {
-        hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
-        /* a wave per column where the units alone nearly fill the card: few pieces each */
-        if (units * 8u >= kWaves)
-            hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3((uint32_t)(units * p.plan.cols)), dim3(64), 0, stream,
-                               p);
-        else
-            hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3((uint32_t)(units * p.plan.cols)), dim3(512), 0, stream,
-                               p);
-    } else {
-        hipLaunchKernelGGL(k_paged_gqa<F>, dim3((uint32_t)((units + 3u) / 4u)), dim3(256), 0, stream, p);
+template <class F> void launch_form(const GqaParams &p, const Launch &L, hipStream_t stream) {
+    const uint32_t pairs = p.c.n_seq * p.c.n_head_kv, units = pairs * p.plan.n_ct, cols = units * p.plan.cols;
+    if (L.how == Launch::kDirect) {
+        hipLaunchKernelGGL(k_paged_gqa<F>, dim3(pairs * ((p.plan.n_ct + 3u) / 4u)), dim3(256), 0, stream, p);
+        return;
     }
+    if constexpr (F::OCC > 1) {
+        if (L.how == Launch::kGroup) {
+            hipLaunchKernelGGL((k_paged_gqa_wg<F, 8>), dim3(units), dim3(512), 0, stream, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
+    /* a unit's pieces: a wave takes 256 / HD at a time, a workgroup of 8 waves 8 times that */
+    if (p.plan.n_waves <= 16u * units)
+        hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3(cols), dim3(64), 0, stream, p);
+    else
+        hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3(cols), dim3(512), 0, stream, p);
 }
 
 } // namespace
@@ -818,14 +896,18 @@ int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int
     p.range         = reinterpret_cast<uint2 *>(w + L.o_bytes + L.ml_bytes);
     if (c.head_dim == 64u) {
         if (L.copies == 4u)
-            launch_form<Form<64, 1, 4, 2>>(p, L.split, stream);
+            launch_form<Form<64, 1, 4, 2, 2>>(p, L, stream);
+        else if (L.tiles == 1u)
+            launch_form<Form<64, 1, 1, 1, 2>>(p, L, stream);
         else
-            launch_form<Form<64, 1, 1, 1>>(p, L.split, stream);
+            launch_form<Form<64, 2, 1, 1, 2>>(p, L, stream);
     } else {
         if (L.copies == 2u)
-            launch_form<Form<128, 1, 2, 1>>(p, L.split, stream);
+            launch_form<Form<128, 1, 2, 1, 2>>(p, L, stream);
+        else if (L.tiles == 1u)
+            launch_form<Form<128, 1, 1, 1, 1>>(p, L, stream);
         else
-            launch_form<Form<128, 1, 1, 1>>(p, L.split, stream);
+            launch_form<Form<128, 2, 1, 1, 1>>(p, L, stream);
     }
     return hip_status(hipGetLastError());
 }
