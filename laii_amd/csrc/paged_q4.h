@@ -56,10 +56,10 @@ LFM_IDX_FN uint32_t lfm_q4_scale(uint32_t head_dim, uint32_t v, uint32_t t, uint
  * row major, cut into tiles of `cols`.  A unit is (sequence, tile, KV head),
  * numbered in that order; its work is the steps of 2^step_shift keys that cover
  * the keys its rows attend.  The batch's N < 2^32 steps, in unit order, go to G
- * waves in equal shares (the first N % G one longer), cut at units; the piece of
- * wave g in unit v has partial slot g + v: along the walk g or v grows, so slots
- * are unique and below G + units.  A unit that one wave covers whole is written
- * directly.  Everything here is 32-bit: a 64-bit division costs a wave more than
+ * waves in equal shares (the first N % G one longer), cut at units.  The pieces
+ * of a workgroup's waves join in LDS; what workgroup g then holds of unit v, if
+ * not all of it, has partial slot g + v: along the walk g or v grows, so slots
+ * are unique and below workgroups + units.  Everything here is 32-bit: a 64-bit division costs a wave more than
  * a step of keys. */
 typedef struct {
     uint32_t n_seq, n_rows, kv_mul, n_head_kv;

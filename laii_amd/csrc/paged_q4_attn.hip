@@ -43,12 +43,50 @@ struct GqaParams {
     float *out;
     int gate_is_logit;
     float scale;
-    /* split: first and last wave of each unit, partial outputs
+    /* split: first and last workgroup of each unit, partial outputs
      * [slot][cols][HD], their (m, l) [slot][cols] */
     uint2 *range;
     float *part_o;
     float2 *part_ml;
 };
+
+/* Sum and maximum over the 4 lanes 16 apart, which share a column: the swaps
+ * give both halves' values to every lane, in whatever order. */
+__device__ __forceinline__ float kg_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x      = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r      = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float kg_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x      = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r      = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ uint32_t kg_max(uint32_t x) {
+    auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x      = max((uint32_t)r[0], (uint32_t)r[1]);
+    r      = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+
+/* x of the lane N further round its row of 16. */
+template <int N> __device__ __forceinline__ float row_ror(float x) {
+    return __uint_as_float(
+        (uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), 0x120 + N, 0xF, 0xF, true));
+}
+/* Sum and maximum over the R copies of a column, 16 / R lanes apart in a row. */
+template <int R> __device__ __forceinline__ float copies_sum(float x) {
+    static_assert(R == 2 || R == 4, "copies");
+    if (R == 4) x += row_ror<4>(x);
+    return x + row_ror<8>(x);
+}
+template <int R> __device__ __forceinline__ float copies_max(float x) {
+    static_assert(R == 2 || R == 4, "copies");
+    if (R == 4) x = fmaxf(x, row_ror<4>(x));
+    return fmaxf(x, row_ror<8>(x));
+}
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
@@ -128,9 +166,9 @@ __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
  * operand is kept R times, zero outside copy r's columns, so that the S product of
  * tile t with copy t % R leaves each column the tile that it takes, with no
  * selection.  NB: blocks of 32 keys per step.  OCC: waves per SIMD that the
- * registers are cut for. */
-template <int HD_, int NT_, int R_, int NB_, int OCC_> struct Form {
-    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_, OCC = OCC_;
+ * registers are cut for.  D: steps that loads run ahead. */
+template <int HD_, int NT_, int R_, int NB_, int OCC_, int D_> struct Form {
+    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_, OCC = OCC_, D = D_;
     static constexpr int G = HD / 32, DT = HD / 16, TILES = 2 * NB, J = TILES / R;
     static constexpr int COLS = R > 1 ? 16 / R : 16 * NT, STEP = 32 * NB;
     static_assert(R == 1 || (NT == 1 && J == 1), "a copy takes one tile per step");
@@ -142,57 +180,58 @@ template <class F> struct Half {
     uint4 s[F::J > 1 ? F::NB : 1][F::G]; /* J 1: .x and .y alone */
 };
 
-/* Wave-uniform place of a step: its one or two blocks, and whether they have
- * pages.  (Members rather than arrays: an array that lanes index moves to LDS.) */
-struct Place {
-    const uint8_t *base0, *base1;
-    bool there0, there1;
-};
-
-/* The table through the scalar cache: no kernel that runs beside this one writes it. */
+/* Wave-uniform values through the scalar cache: no kernel that runs beside this one writes them. */
 typedef const __attribute__((address_space(4))) int32_t *TableRow;
-
-__device__ __forceinline__ bool block_place(const PagedQ4 &c, TableRow table, uint32_t h, uint32_t blk,
-                                            uint32_t block_bytes, const uint8_t **base) {
-    const uint32_t id = (uint32_t)table[blk >> c.blk_shift], in = blk & ((1u << c.blk_shift) - 1u);
-    const bool there  = id < c.n_pages;
-    *base = c.pages + (uint64_t)(there ? id : 0u) * c.page_bytes + (uint64_t)(((h << c.blk_shift) + in) * block_bytes);
-    return there;
+__device__ __forceinline__ uint32_t scalar_at(const uint32_t *a, uint32_t i) {
+    return ((const __attribute__((address_space(4))) uint32_t *)(uintptr_t)a)[i];
 }
 
-template <class F> __device__ __forceinline__ Place place_of(const PagedQ4 &c, TableRow table, uint32_t h, uint32_t step) {
-    Place p;
-    p.there0 = block_place(c, table, h, step * F::NB, 36u * F::HD, &p.base0);
-    p.there1 = p.there0;
-    p.base1  = p.base0;
+/* Page ids of a step's one or two blocks, wave-uniform. */
+struct Ids {
+    uint32_t a, b;
+};
+
+template <class F> __device__ __forceinline__ Ids ids_of(const PagedQ4 &c, TableRow table, uint32_t step) {
+    Ids r;
+    r.a = r.b = (uint32_t)table[(step * F::NB) >> c.blk_shift];
     if (F::NB > 1) { /* a step's last block may lie behind the table: its keys are masked, read the first twice */
         const uint32_t blk = step * F::NB + 1u;
-        p.there1 = block_place(c, table, h, blk * 32u < c.capacity ? blk : blk - 1u, 36u * F::HD, &p.base1);
+        r.b = (uint32_t)table[(blk * 32u < c.capacity ? blk : blk - 1u) >> c.blk_shift];
     }
-    return p;
+    return r;
+}
+
+__device__ __forceinline__ const uint8_t *block_base(const PagedQ4 &c, uint32_t id, uint32_t h, uint32_t blk,
+                                                     uint32_t block_bytes) {
+    const uint32_t in = blk & ((1u << c.blk_shift) - 1u);
+    return c.pages + (uint64_t)(id < c.n_pages ? id : 0u) * c.page_bytes +
+           (uint64_t)(((h << c.blk_shift) + in) * block_bytes);
 }
 
 /* V 0: keys, 1: values. */
-template <class F, int V> __device__ __forceinline__ void load_half(Half<F> &d, const Place &p, uint32_t lane) {
+template <class F, int V>
+__device__ __forceinline__ void load_half(Half<F> &d, const PagedQ4 &c, const Ids &ids, uint32_t h, uint32_t step,
+                                          uint32_t lane) {
     constexpr int HD = F::HD;
-    const uint32_t kg = lane >> 4;
+    const uint32_t kg = lane >> 4, blk = step * F::NB;
+    const uint8_t *base0 = block_base(c, ids.a, h, blk, 36u * HD), *base1 = base0;
+    if (F::NB > 1) base1 = block_base(c, ids.b, h, (blk + 1u) * 32u < c.capacity ? blk + 1u : blk, 36u * HD);
 #pragma unroll
     for (int b = 0; b < F::NB; ++b)
 #pragma unroll
         for (int i = 0; i < HD / 64; ++i)
-            d.c[b][i] = *reinterpret_cast<const uint4 *>((b ? p.base1 : p.base0) + V * 16 * HD + i * 1024 + lane * 16u);
+            d.c[b][i] = *reinterpret_cast<const uint4 *>((b ? base1 : base0) + V * 16 * HD + i * 1024 + lane * 16u);
     if constexpr (F::J > 1) {
 #pragma unroll
         for (int b = 0; b < F::NB; ++b)
 #pragma unroll
             for (int g = 0; g < F::G; ++g)
-                d.s[b][g] =
-                    *reinterpret_cast<const uint4 *>((b ? p.base1 : p.base0) + (32 + 2 * V) * HD + g * 64 +
-                                                     kg * 16u);
+                d.s[b][g] = *reinterpret_cast<const uint4 *>((b ? base1 : base0) + (32 + 2 * V) * HD + g * 64 +
+                                                             kg * 16u);
     } else { /* the 4 keys of this lane's tile */
         const uint32_t u    = (lane & 15u) / (16u / F::R);
-        const int64_t other = F::NB > 1 ? -(int64_t)(u >> 1) & (p.base1 - p.base0) : 0;
-        const uint8_t *base = p.base0 + other + ((32 + 2 * V) * HD + kg * 16u + (u & 1u) * 8u);
+        const int64_t other = F::NB > 1 ? -(int64_t)(u >> 1) & (base1 - base0) : 0;
+        const uint8_t *base = base0 + other + ((32 + 2 * V) * HD + kg * 16u + (u & 1u) * 8u);
 #pragma unroll
         for (int g = 0; g < F::G; ++g) {
             const uint2 a = *reinterpret_cast<const uint2 *>(base + g * 64);
@@ -241,8 +280,7 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
                 x[g][4 * i] = a.x; x[g][4 * i + 1] = a.y; x[g][4 * i + 2] = a.z; x[g][4 * i + 3] = a.w;
                 big = fmaxf(big, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
             }
-        big = fmaxf(big, __shfl_xor(big, 16));
-        big = fmaxf(big, __shfl_xor(big, 32));
+        big = kg_max(big);
         const int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
         const float unit = ldexpf(p.scale < 0.0f ? -1.0f : 1.0f, -e);
 #pragma unroll
@@ -265,9 +303,7 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
                 st.qh[n][r][g] = a.v;
                 st.ql[n][r][g] = z.v;
             }
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            st.c0[n][g] = -72.0f * sum;
+            st.c0[n][g] = -72.0f * kg_sum(sum);
         }
         /* never 0: a masked score is cs * -inf */
         st.cs[n]  = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e), 1e-37f);
@@ -334,13 +370,13 @@ __device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<
  * 0 (weights of masked keys are then 0 whatever was stored). */
 template <class F>
 __device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &v, const State<F> &st,
-                                          const Place &pl, uint32_t key0, uint32_t lane) {
+                                          bool there_a, bool there_b, uint32_t key0, uint32_t lane) {
     constexpr int NT = F::NT, G = F::G, J = F::J;
     const uint32_t kg = lane >> 4, u = (lane & 15u) / (16u / F::R);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const uint32_t t = J > 1 ? (uint32_t)j : u;
-        const bool page  = (pl.there0 || t >= 2u) && (pl.there1 || t < 2u);
+        const bool page  = (there_a || t >= 2u) && (there_b || t < 2u);
         uint32_t keep[2] = {0u, 0u};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -389,17 +425,13 @@ __device__ __forceinline__ void check_step(State<F> &st, const float (&x)[F::NT]
     }
     raise |= dv > st.vmax;
     if (__any(raise)) {
-        dv      = max(dv, (uint32_t)__shfl_xor((int)dv, 16));
-        dv      = max(dv, (uint32_t)__shfl_xor((int)dv, 32));
-        st.vmax = max(dv, st.vmax);
+        st.vmax = max(kg_max(dv), st.vmax);
         /* a scale that is not finite gives NaN in its own dims alone */
         const float z = (float)__builtin_bit_cast(_Float16, (uint16_t)min(st.vmax, 0x7BFFu));
         const float e = (z > 0.0f ? (float)__builtin_amdgcn_frexp_expf(z) : 0.0f) - kLift;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            best[n] = fmaxf(best[n], __shfl_xor(best[n], 16));
-            best[n] = fmaxf(best[n], __shfl_xor(best[n], 32));
-            st.top[n]     = fmaxf(st.top[n], best[n]);
+            st.top[n]     = fmaxf(st.top[n], kg_max(best[n]));
             const float m = st.top[n] + e;
             const float a = __builtin_amdgcn_exp2f(st.m[n] - m);
             st.l[n] *= a;
@@ -461,91 +493,72 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
     }
 }
 
-/* Where a piece stands: the step whose P.V product comes next, and the places
- * of it and of the two behind it. */
-struct Walk {
-    TableRow table;
-    uint32_t h, step, last; /* last: the piece's last step */
-    uint32_t in0, in1;      /* keys that every row of the tile attends */
-    Place at, next, after;
-};
-
-/* One step: its P.V product beside the S product of the next one, neither
- * waiting for the other, while the loads of the next values and of the keys
- * behind the next ones are under way. */
-template <class F>
-__device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk &w, float (&x)[F::NT][4 * F::J],
-                                          float (&y)[F::NT][4 * F::J], Half<F> &v, Half<F> &v_next,
-                                          const Half<F> &k_next, Half<F> &k_after, uint32_t lane, const Magic &mg) {
-    load_half<F, 1>(v_next, w.next, lane);
-    load_half<F, 0>(k_after, w.after, lane);
-    const Place coming  = place_of<F>(p.c, w.table, w.h, w.step + 3u < w.last ? w.step + 3u : w.last);
-    const uint32_t key0 = w.step * F::STEP;
-    if (!(key0 >= w.in0 && key0 + F::STEP <= w.in1 && w.at.there0 && w.at.there1))
-        mask_step<F>(x, v, st, w.at, key0, lane);
-    check_step<F>(st, x, v);
-    scores<F>(y, st, k_next, mg);
-    accumulate<F>(st, x, v, lane, mg);
-    w.at    = w.next;
-    w.next  = w.after;
-    w.after = coming;
-}
-
-/* Steps [a, b) of unit (s, ct, h) into a fresh state.  The first loads go out
- * before the queries are read and split. */
+/* Steps [a, b) of unit (s, ct, h) into a fresh state.  A step's P.V product runs
+ * beside the S product of the next step, neither waiting for the other, while
+ * the values D steps ahead and the keys behind them are loaded; the page ids
+ * come one step before that.  The first loads go out before the queries are read
+ * and split. */
 template <class F>
 __device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
                                           const lfm_q4_tile &t, uint32_t pos0, uint32_t rows, uint32_t a, uint32_t b,
                                           uint32_t lane) {
-    const Magic mg = magic();
-    Walk w;
-    w.table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
-    w.h     = h;
-    w.step  = a;
-    w.last  = b - 1u;
-    w.in0   = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window);
-    w.in1   = pos0 + t.r0 + 1u;
-    w.at    = place_of<F>(p.c, w.table, h, a);
-    w.next  = place_of<F>(p.c, w.table, h, a < w.last ? a + 1u : w.last);
-    w.after = place_of<F>(p.c, w.table, h, a + 2u < w.last ? a + 2u : w.last);
-    Half<F> k0, k1, v0, v1;
-    load_half<F, 0>(k0, w.at, lane);
-    load_half<F, 1>(v0, w.at, lane);
-    load_half<F, 0>(k1, w.next, lane);
+    constexpr uint32_t D = F::D, B = D + 1u; /* buffers: they change roles every step, no copies */
+    const Magic mg       = magic();
+    const TableRow table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
+    const uint32_t last  = b - 1u;
+    /* keys that every row of the tile attends */
+    const uint32_t in0 = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window), in1 = pos0 + t.r0 + 1u;
+    Ids ids[D + 3u]; /* of steps step .. step + D + 2, as far as there are any */
+    Half<F> k[B], v[B];
+#pragma unroll
+    for (uint32_t i = 0; i < D + 2u; ++i) ids[i] = ids_of<F>(p.c, table, a + i < last ? a + i : last);
+    load_half<F, 0>(k[0], p.c, ids[0], h, a, lane);
+    load_half<F, 1>(v[0], p.c, ids[0], h, a, lane);
+#pragma unroll
+    for (uint32_t i = 1; i <= D; ++i) {
+        load_half<F, 0>(k[i % B], p.c, ids[i], h, a + i < last ? a + i : last, lane);
+        if (i < D) load_half<F, 1>(v[i % B], p.c, ids[i], h, a + i < last ? a + i : last, lane);
+    }
     start<F>(st, p, s, ct, h, pos0, rows, lane);
-    float x[F::NT][4 * F::J], y[F::NT][4 * F::J];
-    scores<F>(x, st, k0, mg);
-    for (;;) { /* buffers change roles every step: two steps per turn, no copies */
-        step_once<F>(st, p, w, x, y, v0, v1, k1, k0, lane, mg);
-        if (++w.step == b) break;
-        step_once<F>(st, p, w, y, x, v1, v0, k0, k1, lane, mg);
-        if (++w.step == b) break;
+    float x[F::NT][4 * F::J];
+    scores<F>(x, st, k[0], mg);
+    for (uint32_t step = a;;) {
+#pragma unroll
+        for (uint32_t r = 0; r < B; ++r) {
+            const uint32_t sv = step + D < last ? step + D : last, sk = step + D + 1u < last ? step + D + 1u : last;
+            load_half<F, 1>(v[(r + D) % B], p.c, ids[D], h, sv, lane);
+            load_half<F, 0>(k[r], p.c, ids[D + 1u], h, sk, lane);
+            ids[D + 2u]         = ids_of<F>(p.c, table, step + D + 2u < last ? step + D + 2u : last);
+            const uint32_t key0 = step * F::STEP;
+            const bool there_a = ids[0].a < p.c.n_pages, there_b = ids[0].b < p.c.n_pages;
+            if (!(key0 >= in0 && key0 + F::STEP <= in1 && there_a && there_b))
+                mask_step<F>(x, v[r], st, there_a, there_b, key0, lane);
+            check_step<F>(st, x, v[r]);
+            float y[F::NT][4 * F::J];
+            scores<F>(y, st, k[(r + 1u) % B], mg);
+            accumulate<F>(st, x, v[r], lane, mg);
+#pragma unroll
+            for (int n = 0; n < F::NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4 * F::J; ++i) x[n][i] = y[n][i];
+#pragma unroll
+            for (uint32_t i = 0; i < D + 2u; ++i) ids[i] = ids[i + 1u];
+            if (++step == b) return;
+        }
     }
 }
 
 /* Sums over the lanes that share a column; with R > 1 its copies too. */
 template <class F> __device__ __forceinline__ void join_lanes(State<F> &st) {
 #pragma unroll
-    for (int n = 0; n < F::NT; ++n) {
-        st.l[n] += __shfl_xor(st.l[n], 16);
-        st.l[n] += __shfl_xor(st.l[n], 32);
-    }
+    for (int n = 0; n < F::NT; ++n) st.l[n] = kg_sum(st.l[n]);
     if constexpr (F::R > 1) {
-        float m = st.m[0];
+        const float m = copies_max<F::R>(st.m[0]), a = __builtin_amdgcn_exp2f(st.m[0] - m);
+        st.l[0]       = copies_sum<F::R>(st.l[0] * a);
 #pragma unroll
-        for (int x = 16 / F::R; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
-        const float a = __builtin_amdgcn_exp2f(st.m[0] - m);
-        st.l[0] *= a;
+        for (int i = 0; i < F::DT; ++i)
 #pragma unroll
-        for (int i = 0; i < F::DT; ++i) st.o[0][i] *= a;
-#pragma unroll
-        for (int x = 16 / F::R; x < 16; x *= 2) {
-            st.l[0] += __shfl_xor(st.l[0], x);
-#pragma unroll
-            for (int i = 0; i < F::DT; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) st.o[0][i][k] += __shfl_xor(st.o[0][i][k], x);
-        }
+            for (int k = 0; k < 4; ++k) st.o[0][i][k] = copies_sum<F::R>(st.o[0][i][k] * a);
         st.m[0] = m;
     }
 }
@@ -593,6 +606,11 @@ __device__ __forceinline__ void put_part(const State<F> &st, float *o, float2 *m
     }
 }
 
+/* The same for a wave-uniform s. */
+__device__ __forceinline__ uint32_t rows_at(const PagedQ4 &c, uint32_t s, uint32_t pos0) {
+    return lfm_q4_rows(pos0, c.rows_seq ? scalar_at(c.rows_seq, s) : c.n_rows, c.n_rows, c.capacity);
+}
+
 __device__ __forceinline__ uint32_t rows_of(const PagedQ4 &c, uint32_t s, uint32_t pos0) {
     return lfm_q4_rows(pos0, c.rows_seq ? c.rows_seq[s] : c.n_rows, c.n_rows, c.capacity);
 }
@@ -609,7 +627,7 @@ template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa(co
     const uint32_t back = quad * 4u + uniform(threadIdx.x >> 6);
     if (back >= p.plan.n_ct) return;
     const uint32_t ct   = p.plan.n_ct - 1u - back;
-    const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
+    const uint32_t pos0 = scalar_at(p.c.pos0, s), rows = rows_at(p.c, s, pos0);
     const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
     if (t.n_steps == 0u) return;
     State<F> st;
@@ -618,15 +636,42 @@ template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa(co
     write_out<F>(st, p, s, ct, h, rows, lane);
 }
 
+/* Column col, dims 4 d .. of the pieces at the places in `run` (8 at most). */
+struct Merged {
+    float m, l;
+    float4 o;
+};
+template <class F>
+__device__ __forceinline__ Merged merge_run(const float *so, const float2 *sml, uint32_t run, uint32_t col, uint32_t d) {
+    Merged r = {kNoScore, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    float2 ml[8];
+#pragma unroll
+    for (uint32_t w = 0; w < 8u; ++w) {
+        ml[w] = make_float2(kNoScore, 0.0f);
+        if (run >> w & 1u) ml[w] = sml[w * F::COLS + col];
+        r.m = fmaxf(r.m, ml[w].x);
+    }
+#pragma unroll
+    for (uint32_t w = 0; w < 8u; ++w) {
+        if (!(run >> w & 1u)) continue; /* wave-uniform */
+        const float f  = __builtin_amdgcn_exp2f(ml[w].x - r.m);
+        const float4 x = reinterpret_cast<const float4 *>(so + (w * F::COLS + col) * F::HD)[d];
+        r.l += ml[w].y * f;
+        r.o = make_float4(r.o.x + x.x * f, r.o.y + x.y * f, r.o.z + x.z * f, r.o.w + x.w * f);
+    }
+    return r;
+}
+
 /* One workgroup of W waves per unit: its waves share the steps and join in
  * LDS.  For short units: one launch, no partials. */
 template <class F, int W> __global__ __launch_bounds__(64 * W, 2) void k_paged_gqa_wg(const GqaParams p) {
+    static_assert(W <= 8, "merge_run takes 8 pieces");
     __shared__ __align__(16) float so[W][F::COLS][F::HD];
     __shared__ float2 sml[W][F::COLS];
     const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6);
     const uint32_t unit = blockIdx.x, h = unit % p.c.n_head_kv, sc = unit / p.c.n_head_kv;
     const uint32_t s = sc / p.plan.n_ct, ct = sc - s * p.plan.n_ct;
-    const uint32_t pos0 = uniform(p.c.pos0[s]), rows = uniform(rows_of(p.c, s, pos0));
+    const uint32_t pos0 = scalar_at(p.c.pos0, s), rows = rows_at(p.c, s, pos0);
     const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
     if (t.n_steps == 0u) return;
     uint32_t a, b;
@@ -644,33 +689,17 @@ template <class F, int W> __global__ __launch_bounds__(64 * W, 2) void k_paged_g
         const uint32_t col = i / (F::HD / 4u), d = i % (F::HD / 4u);
         const size_t head  = head_of<F>(p, s, h, rows, ct * F::COLS + col);
         if (head == ~(size_t)0) continue;
-        float m = kNoScore, l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t w = 0; w < parts; ++w) m = fmaxf(m, sml[w][col].x);
-        for (uint32_t w = 0; w < parts; ++w) {
-            const float2 ml = sml[w][col];
-            const float f   = __builtin_amdgcn_exp2f(ml.x - m);
-            const float4 x  = reinterpret_cast<const float4 *>(so[w][col])[d];
-            l += ml.y * f;
-            o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
-        }
-        const float f = out_factor(p, l, head);
-        reinterpret_cast<float4 *>(p.out + head * F::HD)[d] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        const Merged r = merge_run<F>(&so[0][0][0], &sml[0][0], (1u << parts) - 1u, col, d);
+        const float f  = out_factor(p, r.l, head);
+        reinterpret_cast<float4 *>(p.out + head * F::HD)[d] = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
     }
 }
 
-/* Position, rows and steps of entry e (sequence, tile); no steps past the last. */
-struct Entry {
-    uint32_t pos0, rows, steps;
-};
-__device__ __forceinline__ Entry entry_of(const GqaParams &p, uint32_t e, uint32_t n_entries) {
-    Entry r = {0u, 0u, 0u};
-    if (e >= n_entries) return r;
-    const uint32_t s = p.plan.n_ct == 1u ? e : e / p.plan.n_ct;
-    r.pos0           = p.c.pos0[s];
-    r.rows           = rows_of(p.c, s, r.pos0);
-    r.steps          = lfm_q4_tile_of(&p.plan, r.pos0, r.rows, e - s * p.plan.n_ct).n_steps;
-    return r;
+/* Steps of entry e (sequence, tile), none past the last. */
+__device__ __forceinline__ uint32_t steps_of(const GqaParams &p, uint32_t e, uint32_t n_entries) {
+    if (e >= n_entries) return 0u;
+    const uint32_t s = p.plan.n_ct == 1u ? e : e / p.plan.n_ct, pos0 = p.c.pos0[s];
+    return lfm_q4_tile_of(&p.plan, pos0, rows_of(p.c, s, pos0), e - s * p.plan.n_ct).n_steps;
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t lane) { /* inclusive */
@@ -686,23 +715,32 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t i) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)i);
 }
 
-/* Equal shares of the batch's steps per wave. */
+/* Equal shares of the batch's steps per wave.  A wave's first and last piece
+ * may be parts of units; those of the 4 waves of a workgroup join in LDS, and
+ * what is still part of a unit goes to the workspace. */
 template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa_split(const GqaParams p) {
+    __shared__ __align__(16) float so[8][F::COLS][F::HD]; /* first and last piece of each wave */
+    __shared__ float2 sml[8][F::COLS];
+    __shared__ struct {
+        uint32_t unit, s, ct, h, rows, whole; /* unit ~0: none; whole: 1 has the unit's first step, 2 its last */
+    } meta[8];
     const uint32_t lane = threadIdx.x & 63u, nh = p.c.n_head_kv;
-    const uint32_t wave = uniform(blockIdx.x * 4u + (threadIdx.x >> 6));
-    const uint32_t n_e  = p.c.n_seq * p.plan.n_ct;
+    const uint32_t in_wg = uniform(threadIdx.x >> 6), wave = blockIdx.x * 4u + in_wg;
+    const uint32_t n_e = p.c.n_seq * p.plan.n_ct;
+    if (lane < 2u) meta[in_wg * 2u + lane].unit = ~0u;
     /* a window of 64 entries, one per lane; batches of up to 64 keep it */
-    Entry en        = entry_of(p, lane, n_e);
-    uint32_t inc    = wave_scan(en.steps, lane);
-    uint32_t total  = lane_of(inc, 63u);
+    uint32_t inc   = wave_scan(steps_of(p, lane, n_e), lane);
+    uint32_t total = lane_of(inc, 63u);
     for (uint32_t e0 = 64u; e0 < n_e; e0 += 64u)
-        total += lane_of(wave_scan(entry_of(p, e0 + lane, n_e).steps, lane), 63u);
+        total += lane_of(wave_scan(steps_of(p, e0 + lane, n_e), lane), 63u);
     const uint32_t N = total * nh, G = lfm_q4_waves(&p.plan, N);
-    if (wave >= G) return;
-    uint32_t t, t1;
-    lfm_q4_share(wave, N, G, &t, &t1);
-    t  = uniform(t);
-    t1 = uniform(t1);
+    uint32_t t = 0u, t1 = 0u;
+    if (wave < G) {
+        lfm_q4_share(wave, N, G, &t, &t1);
+        t  = uniform(t);
+        t1 = uniform(t1);
+    }
+    const uint32_t t0 = t;
     uint32_t e0 = 0u, base = 0u; /* the window's first entry, steps before it */
     while (t < t1) {
         const uint32_t want = uniform(t / nh);
@@ -710,37 +748,76 @@ template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa_sp
         while (!hit) { /* ends: want is below the total */
             base += lane_of(inc, 63u);
             e0 += 64u;
-            en  = entry_of(p, e0 + lane, n_e);
-            inc = wave_scan(en.steps, lane);
+            inc = wave_scan(steps_of(p, e0 + lane, n_e), lane);
             hit = __ballot(base + inc > want);
         }
         const uint32_t i = (uint32_t)__builtin_ctzll(hit), e = e0 + i;
-        const uint32_t pos0 = lane_of(en.pos0, i), rows = lane_of(en.rows, i), n = lane_of(en.steps, i);
-        const uint32_t first = (base + lane_of(inc, i) - n) * nh;
         const uint32_t s = p.plan.n_ct == 1u ? e : uniform(e / p.plan.n_ct), ct = e - s * p.plan.n_ct;
+        const uint32_t pos0 = scalar_at(p.c.pos0, s), rows = rows_at(p.c, s, pos0);
         const lfm_q4_tile tile = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
+        const uint32_t n = uniform(tile.n_steps), first = (base + lane_of(inc, i) - n) * nh;
         uint32_t h = uniform((t - first) / n);
         uint32_t a = t - first - h * n;
         for (; t < t1 && h < nh; ++h, a = 0u) {
-            const uint32_t b    = n - a < t1 - t ? n : a + (t1 - t);
-            const uint32_t unit = e * nh + h;
+            const uint32_t b = n - a < t1 - t ? n : a + (t1 - t);
             State<F> st;
             run_piece<F>(st, p, s, ct, h, tile, pos0, rows, tile.step0 + a, tile.step0 + b, lane);
             join_lanes<F>(st);
-            if (lane == 0u && a == 0u) p.range[unit].x = wave;
-            if (lane == 0u && b == n) p.range[unit].y = wave;
             if (a == 0u && b == n) {
                 write_out<F>(st, p, s, ct, h, rows, lane);
-            } else {
-                const size_t at = ((size_t)wave + unit) * F::COLS;
-                put_part<F>(st, p.part_o + at * F::HD, p.part_ml + at, lane);
+                if (lane == 0u) p.range[e * nh + h] = make_uint2(blockIdx.x, blockIdx.x);
+            } else { /* the first piece of the share, or its last */
+                const uint32_t at = in_wg * 2u + (t == t0 ? 0u : 1u);
+                put_part<F>(st, &so[at][0][0], &sml[at][0], lane);
+                if (lane == 0u) {
+                    meta[at].unit = e * nh + h;
+                    meta[at].s = s, meta[at].ct = ct, meta[at].h = h, meta[at].rows = rows;
+                    meta[at].whole = (a == 0u ? 1u : 0u) | (b == n ? 2u : 0u);
+                }
             }
             t += b - a;
         }
     }
+    __syncthreads();
+    /* runs of pieces of one unit, with empty places between them */
+    uint32_t units[8], have = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) {
+        units[i] = uniform(meta[i].unit);
+        have |= units[i] != ~0u ? 1u << i : 0u;
+    }
+    while (have) {
+        const uint32_t i = (uint32_t)__builtin_ctz(have), unit = uniform(meta[i].unit);
+        uint32_t run = 0u, whole = 0u;
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k)
+            if ((have >> k & 1u) && units[k] == unit) run |= 1u << k;
+        have &= ~run;
+        whole = uniform(meta[i].whole | meta[31 - __builtin_clz(run)].whole);
+        if (threadIdx.x == 0u) {
+            if (whole & 1u) p.range[unit].x = blockIdx.x;
+            if (whole & 2u) p.range[unit].y = blockIdx.x;
+        }
+        const uint32_t s = meta[i].s, ct = meta[i].ct, h = meta[i].h, rows = meta[i].rows;
+        for (uint32_t x = threadIdx.x; x < F::COLS * F::HD / 4u; x += 256u) {
+            const uint32_t col = x / (F::HD / 4u), d = x % (F::HD / 4u);
+            const Merged r     = merge_run<F>(&so[0][0][0], &sml[0][0], run, col, d);
+            if (whole == 3u) {
+                const size_t head = head_of<F>(p, s, h, rows, ct * F::COLS + col);
+                if (head == ~(size_t)0) continue;
+                const float f = out_factor(p, r.l, head);
+                reinterpret_cast<float4 *>(p.out + head * F::HD)[d] =
+                    make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
+            } else {
+                const size_t at = ((size_t)blockIdx.x + unit) * F::COLS + col;
+                if (d == 0u) p.part_ml[at] = make_float2(r.m, r.l);
+                reinterpret_cast<float4 *>(p.part_o + at * F::HD)[d] = r.o;
+            }
+        }
+    }
 }
 
-/* The pieces of every unit that more than one wave holds: one workgroup per
+/* The pieces of every unit that more than one workgroup holds: one workgroup per
  * (unit, column); HD / 4 threads take a piece, T / (HD / 4) pieces at a time. */
 template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(const GqaParams p) {
     constexpr uint32_t L = HD / 4, P = T / L;
@@ -750,10 +827,12 @@ template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(cons
     const uint32_t unit = blockIdx.x / cols, col = blockIdx.x - unit * cols;
     const uint32_t e = unit / nh, h = unit - e * nh;
     const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
-    const uint2 g       = p.range[unit]; /* not written, and not used, where the column has no row */
+    /* not written, and not used, where the column has no row; what is used is
+     * checked against the launch all the same */
+    const uint2 g = p.range[unit];
     const uint32_t rows = rows_of(p.c, s, p.c.pos0[s]);
     const uint32_t mul = p.plan.kv_mul, ci = ct * cols + col, row = ci / mul;
-    if (row >= rows || g.x == g.y) return;
+    if (row >= rows || g.x >= g.y || g.y >= p.plan.n_waves / 4u) return;
     const uint32_t g0 = g.x, g1 = g.y;
     const size_t head = ((size_t)s * p.c.n_rows + row) * (nh * mul) + h * mul + (ci - row * mul);
     const uint32_t i = threadIdx.x % L, k = threadIdx.x / L;
@@ -833,11 +912,11 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     const uint32_t resident = 4u * kCus * L->occ; /* waves */
     /* enough units fill the card by themselves; step counts of a split are 32 bits */
     L->how = units < 2u * resident && units * (capacity / 32u) < 0x80000000ull ? Launch::kSplit : Launch::kDirect;
-    if (units <= 512u && steps <= kGroupSteps && L->occ == 2u) L->how = Launch::kGroup;
+    if (units <= kCus && steps <= kGroupSteps && L->occ == 2u) L->how = Launch::kGroup;
     uint64_t waves = units * steps;
     if (waves > resident) waves = resident;
     p.n_waves    = (uint32_t)((waves + 3u) / 4u * 4u);
-    const uint64_t slots = L->how == Launch::kSplit ? p.n_waves + units : 0u;
+    const uint64_t slots = L->how == Launch::kSplit ? p.n_waves / 4u + units : 0u;
     L->o_bytes     = slots * p.cols * head_dim * 4u;
     L->ml_bytes    = slots * p.cols * 8u;
     L->range_bytes = L->how == Launch::kSplit ? units * 8u : 0u;
@@ -858,7 +937,7 @@ template <class F> void launch_form(const GqaParams &p, const Launch &L, hipStre
     }
     hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
     /* a unit's pieces: a wave takes 256 / HD at a time, a workgroup of 8 waves 8 times that */
-    if (p.plan.n_waves <= 16u * units)
+    if (p.plan.n_waves / 4u <= 16u * units)
         hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3(cols), dim3(64), 0, stream, p);
     else
         hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3(cols), dim3(512), 0, stream, p);
@@ -896,18 +975,18 @@ int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int
     p.range         = reinterpret_cast<uint2 *>(w + L.o_bytes + L.ml_bytes);
     if (c.head_dim == 64u) {
         if (L.copies == 4u)
-            launch_form<Form<64, 1, 4, 2, 2>>(p, L, stream);
+            launch_form<Form<64, 1, 4, 2, 2, 2>>(p, L, stream);
         else if (L.tiles == 1u)
-            launch_form<Form<64, 1, 1, 1, 2>>(p, L, stream);
+            launch_form<Form<64, 1, 1, 1, 2, 2>>(p, L, stream);
         else
-            launch_form<Form<64, 2, 1, 1, 2>>(p, L, stream);
+            launch_form<Form<64, 2, 1, 1, 2, 1>>(p, L, stream);
     } else {
         if (L.copies == 2u)
-            launch_form<Form<128, 1, 2, 1, 2>>(p, L, stream);
+            launch_form<Form<128, 1, 2, 1, 2, 1>>(p, L, stream);
         else if (L.tiles == 1u)
-            launch_form<Form<128, 1, 1, 1, 1>>(p, L, stream);
+            launch_form<Form<128, 1, 1, 1, 1, 1>>(p, L, stream);
         else
-            launch_form<Form<128, 2, 1, 1, 1>>(p, L, stream);
+            launch_form<Form<128, 2, 1, 1, 1, 1>>(p, L, stream);
     }
     return hip_status(hipGetLastError());
 }
