@@ -90,14 +90,26 @@ template <int R> __device__ __forceinline__ float copies_max(float x) {
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
-/* Constants of the unpacking in vector registers: an and-or takes one scalar operand. */
+/* Constants of the unpacking.  In vector registers: an AND of two vector
+ * registers takes 2.6 cycles of a SIMD with two waves, with a scalar one 4.4. */
 struct Magic {
-    uint32_t b1024, b64;
+    uint32_t low, high; /* nibble 0 and nibble 1 of both halves */
+    half2v up0, up1, less8;
+    float zero; /* keeps p * d one mixed-precision fma */
 };
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
+    uint32_t r;
+    asm("v_mov_b32 %0, %1" : "=v"(r) : "s"(x));
+    return r;
+}
 __device__ __forceinline__ Magic magic() {
     Magic m;
-    asm("v_mov_b32 %0, 0x64006400" : "=v"(m.b1024));
-    asm("v_mov_b32 %0, 0x54005400" : "=v"(m.b64));
+    m.low   = in_vgpr(0x000F000Fu);
+    m.high  = in_vgpr(0x00F000F0u);
+    m.up0   = __builtin_bit_cast(half2v, in_vgpr(0x78007800u)); /* 2^15  */
+    m.up1   = __builtin_bit_cast(half2v, in_vgpr(0x68006800u)); /* 2^11  */
+    m.less8 = __builtin_bit_cast(half2v, in_vgpr(0xA400A400u)); /* -2^-6 */
+    m.zero  = __uint_as_float(in_vgpr(0u));
     return m;
 }
 
@@ -107,53 +119,53 @@ union Words {
     half8v v;
 };
 
-/* The 8 codes of a V word as the A operand of one MFMA, exact: code - 8. */
+/* The 8 codes of a V word as the A operand of one MFMA: 2^-9 (code - 8), exact.
+ * A nibble alone is the fp16 subnormal code * 2^-24 (or 2^-20), so an AND and a
+ * packed fma do: 7.2 cycles a pair where setting an exponent by and-or and
+ * subtracting it takes 9.1. */
+constexpr float kVUp = 512.0f;
 __device__ __forceinline__ half8v unpack_v(uint32_t w, const Magic &k) {
     Words r;
-    const half2v b0 = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    const half2v s1 = {(_Float16)0.0625f, (_Float16)0.0625f}, b1 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const uint32_t x = w >> 8;
-    r.u[0] = (w & 0x000F000Fu) | k.b1024; /* 1024 + code      */
-    r.u[1] = (w & 0x00F000F0u) | k.b1024; /* 1024 + 16 * code */
-    r.u[2] = (x & 0x000F000Fu) | k.b1024;
-    r.u[3] = (x & 0x00F000F0u) | k.b1024;
-    r.h[0] = r.h[0] + b0;
-    r.h[1] = __builtin_elementwise_fma(r.h[1], s1, b1);
-    r.h[2] = r.h[2] + b0;
-    r.h[3] = __builtin_elementwise_fma(r.h[3], s1, b1);
+    r.u[0] = w & k.low;
+    r.u[1] = w & k.high;
+    r.u[2] = x & k.low;
+    r.u[3] = x & k.high;
+    r.h[0] = __builtin_elementwise_fma(r.h[0], k.up0, k.less8);
+    r.h[1] = __builtin_elementwise_fma(r.h[1], k.up1, k.less8);
+    r.h[2] = __builtin_elementwise_fma(r.h[2], k.up0, k.less8);
+    r.h[3] = __builtin_elementwise_fma(r.h[3], k.up1, k.less8);
     return r.v;
 }
 
-/* A K word: elements 0, 1, 4, 5 as code - 8, elements 2, 3, 6, 7 as code + 64.
- * The product with q starts from -72 times the sum of q over the latter, so it
- * is that of code - 8; at 9 times the codes' size fp32 still has bits to spare,
- * which the values' long sums would not have. */
+/* A K word as 2^-20 code: subnormals, as they stand.  The product with q starts
+ * from -8 times the sum of q, so it is that of code - 8; the values' long sums
+ * would lose bits to such an offset, these of 32 terms do not.  (rms error of a
+ * group's product on the matrix unit, of its rms: 7.6e-8 with code - 8, 1.8e-7
+ * with subnormals in bits 6-9, 1.0e-6 with half the codes as code + 64, 4e-6
+ * with subnormals that leave up to 9 bits of the mantissa empty.) */
+constexpr int kKDown = 20;
 __device__ __forceinline__ half8v unpack_k(uint32_t w, const Magic &k) {
     Words r;
-    const half2v b0  = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    const uint32_t x = w >> 8;
-    r.u[0] = (w & 0x000F000Fu) | k.b1024;
-    r.u[1] = (w & 0x00F000F0u) | k.b64;
-    r.u[2] = (x & 0x000F000Fu) | k.b1024;
-    r.u[3] = (x & 0x00F000F0u) | k.b64;
-    r.h[0] = r.h[0] + b0;
-    r.h[2] = r.h[2] + b0;
+    r.u[0] = (w << 4) & k.high;
+    r.u[1] = w & k.high;
+    r.u[2] = (w >> 4) & k.high;
+    r.u[3] = (w >> 8) & k.high;
     return r.v;
 }
 
 __device__ __forceinline__ float half_lo(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[0]; }
 __device__ __forceinline__ float half_hi(uint32_t w) { return (float)__builtin_bit_cast(half2v, w)[1]; }
 
-/* Two weights p * d as fp16 hi + lo: hi is the product rounded, lo what is
- * left of it, rounded; one mixed-precision fma each. */
-__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t d, uint32_t *hi, uint32_t *lo) {
-    half2v h, l;
-    h[0] = (_Float16)fmaf(p0, half_lo(d), 0.0f);
-    h[1] = (_Float16)fmaf(p1, half_hi(d), 0.0f);
-    l[0] = (_Float16)fmaf(p0, half_lo(d), -(float)h[0]);
-    l[1] = (_Float16)fmaf(p1, half_hi(d), -(float)h[1]);
-    *hi  = __builtin_bit_cast(uint32_t, h);
-    *lo  = __builtin_bit_cast(uint32_t, l);
+/* Two weights p * d as fp16 hi + lo: hi is the product truncated, lo what is
+ * left of it, truncated.  (v_fma_mixlo_f16 would round in one instruction, but
+ * takes 8.5 cycles; this takes 28 a pair, that 34.) */
+__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t d, uint32_t *hi, uint32_t *lo,
+                                              const Magic &k) {
+    const float w0 = fmaf(p0, half_lo(d), k.zero), w1 = fmaf(p1, half_hi(d), k.zero);
+    *hi            = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+    const float l0 = fmaf(p0, half_lo(d), -half_lo(*hi)), l1 = fmaf(p1, half_hi(d), -half_hi(*hi));
+    *lo            = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(l0, l1));
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
@@ -244,7 +256,7 @@ __device__ __forceinline__ void load_half(Half<F> &d, const PagedQ4 &c, const Id
 template <class F> struct State {
     half8v qh[F::NT][F::R][F::G], ql[F::NT][F::R][F::G];
     float4v o[F::NT][F::DT];
-    float c0[F::NT][F::G];           /* start of the S product: minus 72 sum q (unpack_k) */
+    float c0[F::NT][F::G];           /* start of the S product: minus 8 sum q (unpack_k) */
     float cs[F::NT], top[F::NT], m[F::NT], l[F::NT];
     uint32_t vmax;                   /* magnitude (fp16 bits) of the V scales that m covers */
     uint32_t lo[F::NT], hi[F::NT];   /* keys [lo, hi) of the column's row */
@@ -292,7 +304,7 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
                 const float y = x[g][i] * unit;
                 yh.v[i]       = (_Float16)y;
                 yl.v[i]       = (_Float16)(y - (float)yh.v[i]);
-                if (i & 2) sum += (float)yh.v[i] + (float)yl.v[i];
+                sum += (float)yh.v[i] + (float)yl.v[i];
             }
 #pragma unroll
             for (int r = 0; r < F::R; ++r) {
@@ -303,10 +315,10 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
                 st.qh[n][r][g] = a.v;
                 st.ql[n][r][g] = z.v;
             }
-            st.c0[n][g] = -72.0f * kg_sum(sum);
+            st.c0[n][g] = ldexpf(-8.0f * kg_sum(sum), -kKDown);
         }
         /* never 0: a masked score is cs * -inf */
-        st.cs[n]  = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e), 1e-37f);
+        st.cs[n]  = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e + kKDown), 1e-37f);
         st.top[n] = st.m[n] = kNoScore;
         st.l[n] = 0.0f;
         st.vmax = 0u;
@@ -447,7 +459,12 @@ template <class F>
 __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F::J], const Half<F> &v,
                                            uint32_t lane, const Magic &mg) {
     constexpr int NT = F::NT, G = F::G, J = F::J, R = F::R;
-    const uint32_t u = (lane & 15u) / (16u / R);
+    uint32_t mine[R]; /* all bits in the lanes of copy r */
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        mine[r] = (lane & 15u) / (16u / R) == (uint32_t)r ? ~0u : 0u;
+        if (R > 1) asm("" : "+v"(mine[r])); /* an AND (2.6 cycles), not a select (4.5) */
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -462,7 +479,7 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
             const uint4 z = v.s[0][g];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                split_weights(x[0][2 * i], x[0][2 * i + 1], i ? z.y : z.x, &ch[i], &cl[i]);
+                split_weights(x[0][2 * i], x[0][2 * i + 1], i ? z.y : z.x, &ch[i], &cl[i], mg);
         }
 #pragma unroll
         for (int b = 0; b < F::NB; ++b) {
@@ -472,12 +489,11 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (R > 1) {
-                        const bool mine = u == (uint32_t)((2 * b + i / 2) % R);
-                        wh[n].u[i]      = mine ? ch[i & 1] : 0u;
-                        wl[n].u[i]      = mine ? cl[i & 1] : 0u;
+                        wh[n].u[i] = ch[i & 1] & mine[(2 * b + i / 2) % R];
+                        wl[n].u[i] = cl[i & 1] & mine[(2 * b + i / 2) % R];
                     } else {
                         split_weights(x[n][8 * b + 2 * i], x[n][8 * b + 2 * i + 1], word_of(v.s[b][g], i),
-                                      &wh[n].u[i], &wl[n].u[i]);
+                                      &wh[n].u[i], &wl[n].u[i], mg);
                     }
                 }
 #pragma unroll
@@ -563,14 +579,15 @@ template <class F> __device__ __forceinline__ void join_lanes(State<F> &st) {
     }
 }
 
-/* 1 / l (0 where no key was attended, NaN where a score was) times the gate. */
+/* 1 / l (0 where no key was attended, NaN where a score was) times the gate,
+ * and what unpack_v left out. */
 __device__ __forceinline__ float out_factor(const GqaParams &p, float l, size_t head) {
     float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
     if (p.gate) {
         const float x = p.gate[head];
         f *= p.gate_is_logit ? 1.0f / (1.0f + expf(-x)) : x;
     }
-    return f;
+    return f * kVUp;
 }
 
 template <class F>
