@@ -31,6 +31,8 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
 constexpr float kNoScore = -1e30f; /* top before any key: finite, so masked scores (-inf) give p = 0 */
 constexpr float kSlack   = 8.0f;   /* log2 by which a score may pass top */
@@ -69,6 +71,16 @@ __device__ __forceinline__ uint32_t kg_max(uint32_t x) {
     x      = max((uint32_t)r[0], (uint32_t)r[1]);
     r      = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+
+/* The same over the two lanes 32 apart. */
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 /* x of the lane N further round its row of 16. */
@@ -168,10 +180,6 @@ __device__ __forceinline__ void split_weights(float p0, float p1, uint32_t d, ui
     *lo            = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(l0, l1));
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
-    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
 /* What one wave computes with.  HD: head_dim.  NT: tiles of 16 query columns.
  * R: with at most 16 / R columns (NT 1), each is held R times, and copy u of it
  * takes every R-th 16-key tile of a step: softmax work shrinks by R.  The query
@@ -183,13 +191,19 @@ template <int HD_, int NT_, int R_, int NB_, int OCC_, int D_> struct Form {
     static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_, OCC = OCC_, D = D_;
     static constexpr int G = HD / 32, DT = HD / 16, TILES = 2 * NB, J = TILES / R;
     static constexpr int COLS = R > 1 ? 16 / R : 16 * NT, STEP = 32 * NB;
+    static constexpr int SB = J > 1 ? NB : 1; /* scales: 8 per block and group, or the 4 of this lane's tile */
+    static constexpr int SW = J > 1 ? 4 : 2;
     static_assert(R == 1 || (NT == 1 && J == 1), "a copy takes one tile per step");
 };
 
-/* One lane's share of a step's codes and scales, keys or values. */
+/* One lane's share of a step's codes and scales, keys or values.  Native
+ * vectors: a load in flight stays one value through the loop (as four, the
+ * compiler moved some at the loop's end, and waited for them to do so). */
 template <class F> struct Half {
-    uint4 c[F::NB][F::HD / 64];
-    uint4 s[F::J > 1 ? F::NB : 1][F::G]; /* J 1: .x and .y alone */
+    uint4v c[F::NB][F::HD / 64];
+    uint4v s[F::SB][F::G * F::SW / 4];
+    /* words i < SW (two fp16 each) of group g of block b */
+    __device__ __forceinline__ uint32_t scales(int b, int g, int i) const { return s[b][(g * F::SW + i) / 4][(g * F::SW + i) % 4]; }
 };
 
 /* Wave-uniform values through the scalar cache: no kernel that runs beside this one writes them. */
@@ -220,6 +234,13 @@ __device__ __forceinline__ const uint8_t *block_base(const PagedQ4 &c, uint32_t 
            (uint64_t)(((h << c.blk_shift) + in) * block_bytes);
 }
 
+/* 16 bytes of codes.  ONCE: a single wave reads them, past the caches (loads
+ * alone, B64 x 16384: 108 -> 94 us). */
+template <bool ONCE> __device__ __forceinline__ uint4v load_codes(const uint8_t *p) {
+    const uint4v *q = reinterpret_cast<const uint4v *>(p);
+    return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+
 /* V 0: keys, 1: values. */
 template <class F, int V>
 __device__ __forceinline__ void load_half(Half<F> &d, const PagedQ4 &c, const Ids &ids, uint32_t h, uint32_t step,
@@ -232,22 +253,23 @@ __device__ __forceinline__ void load_half(Half<F> &d, const PagedQ4 &c, const Id
     for (int b = 0; b < F::NB; ++b)
 #pragma unroll
         for (int i = 0; i < HD / 64; ++i)
-            d.c[b][i] = *reinterpret_cast<const uint4 *>((b ? base1 : base0) + V * 16 * HD + i * 1024 + lane * 16u);
+            d.c[b][i] = load_codes<(F::R > 1)>((b ? base1 : base0) + V * 16 * HD + i * 1024 + lane * 16u);
     if constexpr (F::J > 1) {
 #pragma unroll
         for (int b = 0; b < F::NB; ++b)
 #pragma unroll
             for (int g = 0; g < F::G; ++g)
-                d.s[b][g] = *reinterpret_cast<const uint4 *>((b ? base1 : base0) + (32 + 2 * V) * HD + g * 64 +
-                                                             kg * 16u);
+                d.s[b][g] = *reinterpret_cast<const uint4v *>((b ? base1 : base0) + (32 + 2 * V) * HD + g * 64 +
+                                                              kg * 16u);
     } else { /* the 4 keys of this lane's tile */
         const uint32_t u    = (lane & 15u) / (16u / F::R);
         const int64_t other = F::NB > 1 ? -(int64_t)(u >> 1) & (base1 - base0) : 0;
         const uint8_t *base = base0 + other + ((32 + 2 * V) * HD + kg * 16u + (u & 1u) * 8u);
 #pragma unroll
-        for (int g = 0; g < F::G; ++g) {
-            const uint2 a = *reinterpret_cast<const uint2 *>(base + g * 64);
-            d.s[0][g]     = make_uint4(a.x, a.y, 0u, 0u);
+        for (int g = 0; g < F::G; g += 2) {
+            const uint2v a = __builtin_nontemporal_load(reinterpret_cast<const uint2v *>(base + g * 64));
+            const uint2v z = __builtin_nontemporal_load(reinterpret_cast<const uint2v *>(base + g * 64 + 64));
+            d.s[0][g / 2]  = __builtin_shufflevector(a, z, 0, 1, 2, 3);
         }
     }
 }
@@ -352,7 +374,7 @@ __device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const uint32_t w =
-                    F::HD == 64 ? word_of(k.c[b][0], half * 2 + g) : word_of(k.c[b][half % (F::HD / 64)], g);
+                    F::HD == 64 ? k.c[b][0][half * 2 + g % 2] : k.c[b][half % (F::HD / 64)][g];
                 const half8v a = unpack_k(w, mg);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -369,7 +391,7 @@ __device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<
                 float y = 0.0f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const uint32_t z = word_of(k.s[b][g], w0 + i / 2);
+                    const uint32_t z = k.scales(b, g, w0 + i / 2);
                     y                = fmaf(i & 1 ? half_hi(z) : half_lo(z), acc[n][g][i], y);
                 }
                 x[n][4 * j + i] = y;
@@ -404,11 +426,10 @@ __device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            uint4 &z = v.s[J > 1 ? j / 2 : 0][g];
-            if (J > 1 && (j & 1))
-                z.z &= keep[0], z.w &= keep[1];
-            else
-                z.x &= keep[0], z.y &= keep[1];
+            const int w = J > 1 ? (j & 1) * 2 : 0;
+            const int at = g * F::SW + w;
+            v.s[J > 1 ? j / 2 : 0][at / 4][at % 4] &= keep[0];
+            v.s[J > 1 ? j / 2 : 0][at / 4][at % 4 + 1] &= keep[1];
         }
     }
 }
@@ -421,11 +442,11 @@ __device__ __forceinline__ void check_step(State<F> &st, const float (&x)[F::NT]
     uint32_t dv = 0u;
     bool raise  = false;
 #pragma unroll
-    for (int b = 0; b < (J > 1 ? F::NB : 1); ++b)
+    for (int b = 0; b < F::SB; ++b)
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int i = 0; i < (J > 1 ? 4 : 2); ++i) dv = pk_max_u16(dv, word_of(v.s[b][g], i) & 0x7FFF7FFFu);
+            for (int i = 0; i < F::SW; ++i) dv = pk_max_u16(dv, v.scales(b, g, i) & 0x7FFF7FFFu);
     dv = max(dv & 0xFFFFu, dv >> 16);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -476,10 +497,9 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
     for (int g = 0; g < G; ++g) {
         uint32_t ch[2], cl[2]; /* R > 1: this lane's 4 keys */
         if constexpr (R > 1) {
-            const uint4 z = v.s[0][g];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                split_weights(x[0][2 * i], x[0][2 * i + 1], i ? z.y : z.x, &ch[i], &cl[i], mg);
+                split_weights(x[0][2 * i], x[0][2 * i + 1], v.scales(0, g, i), &ch[i], &cl[i], mg);
         }
 #pragma unroll
         for (int b = 0; b < F::NB; ++b) {
@@ -492,13 +512,13 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
                         wh[n].u[i] = ch[i & 1] & mine[(2 * b + i / 2) % R];
                         wl[n].u[i] = cl[i & 1] & mine[(2 * b + i / 2) % R];
                     } else {
-                        split_weights(x[n][8 * b + 2 * i], x[n][8 * b + 2 * i + 1], word_of(v.s[b][g], i),
+                        split_weights(x[n][8 * b + 2 * i], x[n][8 * b + 2 * i + 1], v.scales(b, g, i),
                                       &wh[n].u[i], &wl[n].u[i], mg);
                     }
                 }
 #pragma unroll
             for (int i = 2 * g; i < 2 * g + 2; ++i) {
-                const half8v a = unpack_v(word_of(v.c[b][i / 4], i & 3), mg);
+                const half8v a = unpack_v(v.c[b][i / 4][i & 3], mg);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     st.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[n].v, st.o[n][i], 0, 0, 0);
@@ -509,59 +529,83 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
     }
 }
 
-/* Steps [a, b) of unit (s, ct, h) into a fresh state.  A step's P.V product runs
- * beside the S product of the next step, neither waiting for the other, while
- * the values D steps ahead and the keys behind them are loaded; the page ids
- * come one step before that.  The first loads go out before the queries are read
- * and split. */
+/* Where a piece stands, wave-uniform. */
+template <class F> struct Walk {
+    TableRow table;
+    uint32_t h, step, last; /* last: the piece's last step */
+    uint32_t in0, in1;      /* keys that every row of the tile attends */
+    Ids ids[F::D + 3];      /* of steps step .. step + D + 2, as far as there are any */
+};
+
+/* One step: its P.V product beside the S product of the next step, neither
+ * waiting for the other.  LOAD: while the values D steps ahead and the keys
+ * behind them are loaded; the page ids come one step before that. */
+template <class F, bool LOAD>
+__device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk<F> &w, float (&x)[F::NT][4 * F::J],
+                                          Half<F> &v, Half<F> &v_new, const Half<F> &k_next, Half<F> &k_new,
+                                          uint32_t lane, const Magic &mg) {
+    constexpr uint32_t D = F::D;
+    if constexpr (LOAD) {
+        load_half<F, 1>(v_new, p.c, w.ids[D], w.h, w.step + D < w.last ? w.step + D : w.last, lane);
+        load_half<F, 0>(k_new, p.c, w.ids[D + 1u], w.h, w.step + D + 1u < w.last ? w.step + D + 1u : w.last, lane);
+        w.ids[D + 2u] = ids_of<F>(p.c, w.table, w.step + D + 2u < w.last ? w.step + D + 2u : w.last);
+    }
+    const uint32_t key0 = w.step * F::STEP;
+    const bool there_a = w.ids[0].a < p.c.n_pages, there_b = w.ids[0].b < p.c.n_pages;
+    if (!(key0 >= w.in0 && key0 + F::STEP <= w.in1 && there_a && there_b))
+        mask_step<F>(x, v, st, there_a, there_b, key0, lane);
+    check_step<F>(st, x, v);
+    float y[F::NT][4 * F::J];
+    scores<F>(y, st, k_next, mg);
+    accumulate<F>(st, x, v, lane, mg);
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4 * F::J; ++i) x[n][i] = y[n][i];
+#pragma unroll
+    for (uint32_t i = 0; i < D + 2u; ++i) w.ids[i] = w.ids[i + 1u];
+    ++w.step;
+}
+
+/* Steps [a, b) of unit (s, ct, h) into a fresh state.  Buffers change roles every
+ * step, so D + 1 steps make a turn without copies; the steps that do not fill a
+ * turn come after the loop, which so has one way out (with one per step, values
+ * met there in new registers, and every turn waited for its last loads).  The
+ * first loads go out before the queries are read and split. */
 template <class F>
 __device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
                                           const lfm_q4_tile &t, uint32_t pos0, uint32_t rows, uint32_t a, uint32_t b,
                                           uint32_t lane) {
-    constexpr uint32_t D = F::D, B = D + 1u; /* buffers: they change roles every step, no copies */
-    const Magic mg       = magic();
-    const TableRow table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
-    const uint32_t last  = b - 1u;
-    /* keys that every row of the tile attends */
-    const uint32_t in0 = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window), in1 = pos0 + t.r0 + 1u;
-    Ids ids[D + 3u]; /* of steps step .. step + D + 2, as far as there are any */
+    constexpr uint32_t D = F::D, B = D + 1u;
+    const Magic mg = magic();
+    Walk<F> w;
+    w.table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
+    w.h     = h;
+    w.step  = a;
+    w.last  = b - 1u;
+    w.in0   = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window);
+    w.in1   = pos0 + t.r0 + 1u;
     Half<F> k[B], v[B];
 #pragma unroll
-    for (uint32_t i = 0; i < D + 2u; ++i) ids[i] = ids_of<F>(p.c, table, a + i < last ? a + i : last);
-    load_half<F, 0>(k[0], p.c, ids[0], h, a, lane);
-    load_half<F, 1>(v[0], p.c, ids[0], h, a, lane);
+    for (uint32_t i = 0; i < D + 2u; ++i) w.ids[i] = ids_of<F>(p.c, w.table, a + i < w.last ? a + i : w.last);
+    load_half<F, 0>(k[0], p.c, w.ids[0], h, a, lane);
+    load_half<F, 1>(v[0], p.c, w.ids[0], h, a, lane);
 #pragma unroll
     for (uint32_t i = 1; i <= D; ++i) {
-        load_half<F, 0>(k[i % B], p.c, ids[i], h, a + i < last ? a + i : last, lane);
-        if (i < D) load_half<F, 1>(v[i % B], p.c, ids[i], h, a + i < last ? a + i : last, lane);
+        load_half<F, 0>(k[i % B], p.c, w.ids[i], h, a + i < w.last ? a + i : w.last, lane);
+        if (i < D) load_half<F, 1>(v[i % B], p.c, w.ids[i], h, a + i < w.last ? a + i : w.last, lane);
     }
     start<F>(st, p, s, ct, h, pos0, rows, lane);
     float x[F::NT][4 * F::J];
     scores<F>(x, st, k[0], mg);
-    for (uint32_t step = a;;) {
+    while (w.step + B <= b) {
 #pragma unroll
-        for (uint32_t r = 0; r < B; ++r) {
-            const uint32_t sv = step + D < last ? step + D : last, sk = step + D + 1u < last ? step + D + 1u : last;
-            load_half<F, 1>(v[(r + D) % B], p.c, ids[D], h, sv, lane);
-            load_half<F, 0>(k[r], p.c, ids[D + 1u], h, sk, lane);
-            ids[D + 2u]         = ids_of<F>(p.c, table, step + D + 2u < last ? step + D + 2u : last);
-            const uint32_t key0 = step * F::STEP;
-            const bool there_a = ids[0].a < p.c.n_pages, there_b = ids[0].b < p.c.n_pages;
-            if (!(key0 >= in0 && key0 + F::STEP <= in1 && there_a && there_b))
-                mask_step<F>(x, v[r], st, there_a, there_b, key0, lane);
-            check_step<F>(st, x, v[r]);
-            float y[F::NT][4 * F::J];
-            scores<F>(y, st, k[(r + 1u) % B], mg);
-            accumulate<F>(st, x, v[r], lane, mg);
-#pragma unroll
-            for (int n = 0; n < F::NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4 * F::J; ++i) x[n][i] = y[n][i];
-#pragma unroll
-            for (uint32_t i = 0; i < D + 2u; ++i) ids[i] = ids[i + 1u];
-            if (++step == b) return;
-        }
+        for (uint32_t r = 0; r < B; ++r)
+            step_once<F, true>(st, p, w, x, v[r], v[(r + D) % B], k[(r + 1u) % B], k[r], lane, mg);
     }
+#pragma unroll
+    for (uint32_t r = 0; r < D; ++r)
+        if (w.step < b) step_once<F, false>(st, p, w, x, v[r], v[r], k[(r + 1u) % B], k[r], lane, mg);
 }
 
 /* Sums over the lanes that share a column; with R > 1 its copies too. */
@@ -834,25 +878,27 @@ template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa_sp
     }
 }
 
-/* The pieces of every unit that more than one workgroup holds: one workgroup per
- * (unit, column); HD / 4 threads take a piece, T / (HD / 4) pieces at a time. */
-template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(const GqaParams p) {
+/* The pieces of the units that more than one workgroup holds: an item is a
+ * (unit, column), HD / 4 threads take a piece.  T 64: a wave per item, 4 in a
+ * workgroup, which meet in registers: for few pieces.  Else T threads per item,
+ * which meet in LDS.  Per piece and column (m, l) and HD floats are read. */
+template <int HD, int T> __global__ __launch_bounds__(T < 256 ? 256 : T) void k_paged_merge(const GqaParams p) {
     constexpr uint32_t L = HD / 4, P = T / L;
-    __shared__ float sm[P], sl[P];
-    __shared__ float4 so[P][L];
     const uint32_t nh = p.c.n_head_kv, cols = p.plan.cols;
-    const uint32_t unit = blockIdx.x / cols, col = blockIdx.x - unit * cols;
+    const uint32_t item = T < 256 ? blockIdx.x * 4u + uniform(threadIdx.x >> 6) : blockIdx.x;
+    const uint32_t unit = item / cols, col = item - unit * cols;
     const uint32_t e = unit / nh, h = unit - e * nh;
     const uint32_t s = e / p.plan.n_ct, ct = e - s * p.plan.n_ct;
+    if (s >= p.c.n_seq) return;
     /* not written, and not used, where the column has no row; what is used is
      * checked against the launch all the same */
-    const uint2 g = p.range[unit];
+    const uint2 g       = p.range[unit];
     const uint32_t rows = rows_of(p.c, s, p.c.pos0[s]);
     const uint32_t mul = p.plan.kv_mul, ci = ct * cols + col, row = ci / mul;
     if (row >= rows || g.x >= g.y || g.y >= p.plan.n_waves / 4u) return;
     const uint32_t g0 = g.x, g1 = g.y;
     const size_t head = ((size_t)s * p.c.n_rows + row) * (nh * mul) + h * mul + (ci - row * mul);
-    const uint32_t i = threadIdx.x % L, k = threadIdx.x / L;
+    const uint32_t t = T < 256 ? threadIdx.x & 63u : threadIdx.x, i = t % L, k = t / L;
     float m = kNoScore, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (uint32_t w = g0 + k; w <= g1; w += P) {
@@ -864,24 +910,36 @@ template <int HD, int T> __global__ __launch_bounds__(T) void k_paged_merge(cons
         l = l * a + ml.y * b;
         o = make_float4(o.x * a + x.x * b, o.y * a + x.y * b, o.z * a + x.z * b, o.w * a + x.w * b);
     }
-    so[k][i] = o;
-    if (i == 0u) sm[k] = m, sl[k] = l;
-    __syncthreads();
-    if (k != 0u) return;
-    float mm = m;
+    if constexpr (T < 256) { /* P is 4 or 2: the lanes 16 or 32 apart */
+        const float mm = P == 4 ? kg_max(m) : pair_max(m), f = __builtin_amdgcn_exp2f(m - mm);
+        l              = P == 4 ? kg_sum(l * f) : pair_sum(l * f);
+        o.x            = P == 4 ? kg_sum(o.x * f) : pair_sum(o.x * f);
+        o.y            = P == 4 ? kg_sum(o.y * f) : pair_sum(o.y * f);
+        o.z            = P == 4 ? kg_sum(o.z * f) : pair_sum(o.z * f);
+        o.w            = P == 4 ? kg_sum(o.w * f) : pair_sum(o.w * f);
+    } else {
+        __shared__ float sm[P], sl[P];
+        __shared__ float4 so[P][L];
+        so[k][i] = o;
+        if (i == 0u) sm[k] = m, sl[k] = l;
+        __syncthreads();
+        if (k != 0u) return;
+        float mm = m;
 #pragma unroll
-    for (uint32_t j = 1; j < P; ++j) mm = fmaxf(mm, sm[j]);
-    float ll = 0.0f;
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t j = 1; j < P; ++j) mm = fmaxf(mm, sm[j]);
+        l = 0.0f;
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (uint32_t j = 0; j < P; ++j) {
-        const float b = __builtin_amdgcn_exp2f(sm[j] - mm);
-        const float4 x = so[j][i];
-        ll += sl[j] * b;
-        o = make_float4(o.x + x.x * b, o.y + x.y * b, o.z + x.z * b, o.w + x.w * b);
+        for (uint32_t j = 0; j < P; ++j) {
+            const float b  = __builtin_amdgcn_exp2f(sm[j] - mm);
+            const float4 x = so[j][i];
+            l += sl[j] * b;
+            o = make_float4(o.x + x.x * b, o.y + x.y * b, o.z + x.z * b, o.w + x.w * b);
+        }
     }
-    const float f = out_factor(p, ll, head);
-    reinterpret_cast<float4 *>(p.out + head * HD)[i] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    const float f = out_factor(p, l, head);
+    if (k == 0u)
+        reinterpret_cast<float4 *>(p.out + head * HD)[i] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 }
 
 /* ---- host: forms, split, scratch ------------------------------------------------ */
@@ -955,7 +1013,7 @@ template <class F> void launch_form(const GqaParams &p, const Launch &L, hipStre
     hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
     /* a unit's pieces: a wave takes 256 / HD at a time, a workgroup of 8 waves 8 times that */
     if (p.plan.n_waves / 4u <= 16u * units)
-        hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3(cols), dim3(64), 0, stream, p);
+        hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3((cols + 3u) / 4u), dim3(256), 0, stream, p);
     else
         hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3(cols), dim3(512), 0, stream, p);
 }
@@ -992,7 +1050,7 @@ int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int
     p.range         = reinterpret_cast<uint2 *>(w + L.o_bytes + L.ml_bytes);
     if (c.head_dim == 64u) {
         if (L.copies == 4u)
-            launch_form<Form<64, 1, 4, 2, 2, 2>>(p, L, stream);
+            launch_form<Form<64, 1, 4, 2, 2, 1>>(p, L, stream);
         else if (L.tiles == 1u)
             launch_form<Form<64, 1, 1, 1, 2, 2>>(p, L, stream);
         else
