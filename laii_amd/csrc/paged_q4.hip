@@ -217,9 +217,11 @@ __device__ __forceinline__ uint32_t half_of(uint32_t code, float d) {
     return __builtin_bit_cast(uint16_t, (_Float16)(d * ((float)code - 8.0f)));
 }
 
-/* One workgroup per (sequence, block, KV head): 8 dims of a position per
- * thread and pass.  Keys come a word at a time; values are nibbles of 8 words. */
+/* One workgroup per (sequence, block, KV head).  The block comes to LDS whole, in
+ * 16-byte loads; a thread then unpacks 8 dims of a position: of the keys one
+ * word, of the values a nibble of each of 8 words. */
 template <int HD> __global__ __launch_bounds__(256) void k_paged_gather(const GatherParams p) {
+    __shared__ __align__(16) uint8_t blk_lds[36 * HD];
     const PagedQ4 &c = p.c;
     const uint32_t h = blockIdx.x % c.n_head_kv, rest = blockIdx.x / c.n_head_kv;
     const uint32_t s = rest / p.n_blk, bi = rest - s * p.n_blk;
@@ -228,35 +230,31 @@ template <int HD> __global__ __launch_bounds__(256) void k_paged_gather(const Ga
     const uint32_t blk = pos0 / 32u + bi;
     if (blk > (pos0 + rows - 1u) / 32u) return;
     const uint8_t *base = block_at(c, s, blk, h);
+    for (uint32_t i = threadIdx.x; i < 36u * HD / 16u; i += 256u)
+        reinterpret_cast<uint4 *>(blk_lds)[i] = base ? reinterpret_cast<const uint4 *>(base)[i] : make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads(); /* without a page: scales 0, so zeros */
     const uint32_t t0 = bi == 0u ? pos0 % 32u : 0u;
     const uint32_t t1 = min(32u, pos0 + rows - blk * 32u);
     for (uint32_t w = threadIdx.x; w < 4u * HD; w += 256u) {
         const uint32_t t = w / (HD / 8), part = w % (HD / 8), g = part / 4u;
         if (t < t0 || t >= t1) continue;
-        uint4 ko = make_uint4(0u, 0u, 0u, 0u), vo = ko;
-        if (base) {
-            const uint32_t kw = *reinterpret_cast<const uint32_t *>(base + lfm_q4_k_word(HD, t, g, part & 3u));
-            const float kd =
-                (float)*reinterpret_cast<const _Float16 *>(base + lfm_q4_scale(HD, 0u, t, g));
-            const float vd =
-                (float)*reinterpret_cast<const _Float16 *>(base + lfm_q4_scale(HD, 1u, t, g));
-            const uint32_t vs = 4u * lfm_q4_nibble(lfm_q4_elem(t));
-            uint32_t k[4], v[4];
+        const uint32_t kw = *reinterpret_cast<const uint32_t *>(blk_lds + lfm_q4_k_word(HD, t, g, part & 3u));
+        const float kd = (float)*reinterpret_cast<const _Float16 *>(blk_lds + lfm_q4_scale(HD, 0u, t, g));
+        const float vd = (float)*reinterpret_cast<const _Float16 *>(blk_lds + lfm_q4_scale(HD, 1u, t, g));
+        const uint32_t vs = 4u * lfm_q4_nibble(lfm_q4_elem(t));
+        uint32_t k[4], v[4];
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) {
-                const uint32_t vw =
-                    *reinterpret_cast<const uint32_t *>(base + lfm_q4_v_word(HD, lfm_q4_kg(t), 8u * part + e));
-                const uint32_t a = half_of((kw >> (4u * lfm_q4_nibble(e))) & 15u, kd);
-                const uint32_t b = half_of((vw >> vs) & 15u, vd);
-                k[e / 2u] = e & 1u ? k[e / 2u] | a << 16 : a;
-                v[e / 2u] = e & 1u ? v[e / 2u] | b << 16 : b;
-            }
-            ko = make_uint4(k[0], k[1], k[2], k[3]);
-            vo = make_uint4(v[0], v[1], v[2], v[3]);
+        for (uint32_t e = 0; e < 8u; ++e) {
+            const uint32_t vw =
+                *reinterpret_cast<const uint32_t *>(blk_lds + lfm_q4_v_word(HD, lfm_q4_kg(t), 8u * part + e));
+            const uint32_t a = half_of((kw >> (4u * lfm_q4_nibble(e))) & 15u, kd);
+            const uint32_t b = half_of((vw >> vs) & 15u, vd);
+            k[e / 2u] = e & 1u ? k[e / 2u] | a << 16 : a;
+            v[e / 2u] = e & 1u ? v[e / 2u] | b << 16 : b;
         }
         const size_t at = (((size_t)s * c.n_rows + (blk * 32u + t - pos0)) * c.n_head_kv + h) * (HD / 8) + part;
-        reinterpret_cast<uint4 *>(p.k_out)[at] = ko;
-        reinterpret_cast<uint4 *>(p.v_out)[at] = vo;
+        reinterpret_cast<uint4 *>(p.k_out)[at] = make_uint4(k[0], k[1], k[2], k[3]);
+        reinterpret_cast<uint4 *>(p.v_out)[at] = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
 

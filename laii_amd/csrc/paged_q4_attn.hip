@@ -185,10 +185,10 @@ __device__ __forceinline__ void split_weights(float p0, float p1, uint32_t d, ui
  * takes every R-th 16-key tile of a step: softmax work shrinks by R.  The query
  * operand is kept R times, zero outside copy r's columns, so that the S product of
  * tile t with copy t % R leaves each column the tile that it takes, with no
- * selection.  NB: blocks of 32 keys per step.  OCC: waves per SIMD that the
- * registers are cut for.  D: steps that loads run ahead. */
-template <int HD_, int NT_, int R_, int NB_, int OCC_, int D_> struct Form {
-    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_, OCC = OCC_, D = D_;
+ * selection.  NB: blocks of 32 keys per step.  Registers are cut for two waves
+ * per SIMD. */
+template <int HD_, int NT_, int R_, int NB_> struct Form {
+    static constexpr int HD = HD_, NT = NT_, R = R_, NB = NB_;
     static constexpr int G = HD / 32, DT = HD / 16, TILES = 2 * NB, J = TILES / R;
     static constexpr int COLS = R > 1 ? 16 / R : 16 * NT, STEP = 32 * NB;
     static constexpr int SB = J > 1 ? NB : 1; /* scales: 8 per block and group, or the 4 of this lane's tile */
@@ -530,25 +530,25 @@ __device__ __forceinline__ void accumulate(State<F> &st, float (&x)[F::NT][4 * F
 }
 
 /* Where a piece stands, wave-uniform. */
-template <class F> struct Walk {
+struct Walk {
     TableRow table;
     uint32_t h, step, last; /* last: the piece's last step */
     uint32_t in0, in1;      /* keys that every row of the tile attends */
-    Ids ids[F::D + 3];      /* of steps step .. step + D + 2, as far as there are any */
+    Ids ids[4];             /* of steps step .. step + 3, as far as there are any */
 };
 
 /* One step: its P.V product beside the S product of the next step, neither
- * waiting for the other.  LOAD: while the values D steps ahead and the keys
- * behind them are loaded; the page ids come one step before that. */
+ * waiting for the other.  LOAD: while the next values and the keys behind the
+ * next ones are loaded; the page ids come one step before that.  (Loads one step
+ * further ahead were no faster.) */
 template <class F, bool LOAD>
-__device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk<F> &w, float (&x)[F::NT][4 * F::J],
+__device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk &w, float (&x)[F::NT][4 * F::J],
                                           Half<F> &v, Half<F> &v_new, const Half<F> &k_next, Half<F> &k_new,
                                           uint32_t lane, const Magic &mg) {
-    constexpr uint32_t D = F::D;
     if constexpr (LOAD) {
-        load_half<F, 1>(v_new, p.c, w.ids[D], w.h, w.step + D < w.last ? w.step + D : w.last, lane);
-        load_half<F, 0>(k_new, p.c, w.ids[D + 1u], w.h, w.step + D + 1u < w.last ? w.step + D + 1u : w.last, lane);
-        w.ids[D + 2u] = ids_of<F>(p.c, w.table, w.step + D + 2u < w.last ? w.step + D + 2u : w.last);
+        load_half<F, 1>(v_new, p.c, w.ids[1], w.h, w.step + 1u < w.last ? w.step + 1u : w.last, lane);
+        load_half<F, 0>(k_new, p.c, w.ids[2], w.h, w.step + 2u < w.last ? w.step + 2u : w.last, lane);
+        w.ids[3] = ids_of<F>(p.c, w.table, w.step + 3u < w.last ? w.step + 3u : w.last);
     }
     const uint32_t key0 = w.step * F::STEP;
     const bool there_a = w.ids[0].a < p.c.n_pages, there_b = w.ids[0].b < p.c.n_pages;
@@ -563,49 +563,41 @@ __device__ __forceinline__ void step_once(State<F> &st, const GqaParams &p, Walk
 #pragma unroll
         for (int i = 0; i < 4 * F::J; ++i) x[n][i] = y[n][i];
 #pragma unroll
-    for (uint32_t i = 0; i < D + 2u; ++i) w.ids[i] = w.ids[i + 1u];
+    for (uint32_t i = 0; i < 3u; ++i) w.ids[i] = w.ids[i + 1u];
     ++w.step;
 }
 
 /* Steps [a, b) of unit (s, ct, h) into a fresh state.  Buffers change roles every
- * step, so D + 1 steps make a turn without copies; the steps that do not fill a
- * turn come after the loop, which so has one way out (with one per step, values
- * met there in new registers, and every turn waited for its last loads).  The
- * first loads go out before the queries are read and split. */
+ * step, so two steps make a turn without copies; an odd last step comes after
+ * the loop, which so has one way out (with one per step, values met there in new
+ * registers, and every turn waited for its last loads).  The first loads go out
+ * before the queries are read and split. */
 template <class F>
 __device__ __forceinline__ void run_piece(State<F> &st, const GqaParams &p, uint32_t s, uint32_t ct, uint32_t h,
                                           const lfm_q4_tile &t, uint32_t pos0, uint32_t rows, uint32_t a, uint32_t b,
                                           uint32_t lane) {
-    constexpr uint32_t D = F::D, B = D + 1u;
     const Magic mg = magic();
-    Walk<F> w;
+    Walk w;
     w.table = (TableRow)(uintptr_t)(p.c.table + (size_t)s * p.c.table_stride);
     w.h     = h;
     w.step  = a;
     w.last  = b - 1u;
     w.in0   = lfm_q4_row_lo(pos0 + t.r1 - 1u, p.plan.window);
     w.in1   = pos0 + t.r0 + 1u;
-    Half<F> k[B], v[B];
+    Half<F> k0, k1, v0, v1;
 #pragma unroll
-    for (uint32_t i = 0; i < D + 2u; ++i) w.ids[i] = ids_of<F>(p.c, w.table, a + i < w.last ? a + i : w.last);
-    load_half<F, 0>(k[0], p.c, w.ids[0], h, a, lane);
-    load_half<F, 1>(v[0], p.c, w.ids[0], h, a, lane);
-#pragma unroll
-    for (uint32_t i = 1; i <= D; ++i) {
-        load_half<F, 0>(k[i % B], p.c, w.ids[i], h, a + i < w.last ? a + i : w.last, lane);
-        if (i < D) load_half<F, 1>(v[i % B], p.c, w.ids[i], h, a + i < w.last ? a + i : w.last, lane);
-    }
+    for (uint32_t i = 0; i < 3u; ++i) w.ids[i] = ids_of<F>(p.c, w.table, a + i < w.last ? a + i : w.last);
+    load_half<F, 0>(k0, p.c, w.ids[0], h, a, lane);
+    load_half<F, 1>(v0, p.c, w.ids[0], h, a, lane);
+    load_half<F, 0>(k1, p.c, w.ids[1], h, a + 1u < w.last ? a + 1u : w.last, lane);
     start<F>(st, p, s, ct, h, pos0, rows, lane);
     float x[F::NT][4 * F::J];
-    scores<F>(x, st, k[0], mg);
-    while (w.step + B <= b) {
-#pragma unroll
-        for (uint32_t r = 0; r < B; ++r)
-            step_once<F, true>(st, p, w, x, v[r], v[(r + D) % B], k[(r + 1u) % B], k[r], lane, mg);
+    scores<F>(x, st, k0, mg);
+    while (w.step + 2u <= b) {
+        step_once<F, true>(st, p, w, x, v0, v1, k1, k0, lane, mg);
+        step_once<F, true>(st, p, w, x, v1, v0, k0, k1, lane, mg);
     }
-#pragma unroll
-    for (uint32_t r = 0; r < D; ++r)
-        if (w.step < b) step_once<F, false>(st, p, w, x, v[r], v[r], k[(r + 1u) % B], k[r], lane, mg);
+    if (w.step < b) step_once<F, false>(st, p, w, x, v0, v1, k1, k0, lane, mg);
 }
 
 /* Sums over the lanes that share a column; with R > 1 its copies too. */
@@ -681,7 +673,7 @@ __device__ __forceinline__ uint32_t rows_of(const PagedQ4 &c, uint32_t s, uint32
  * tiles, with the most keys, are dispatched first; consecutive workgroups, which
  * go to the 8 XCDs in turn, differ in KV head, so a head's pages mostly stay in
  * one XCD's L2. */
-template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa(const GqaParams p) {
+template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa(const GqaParams p) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t pairs = p.c.n_seq * p.c.n_head_kv, quad = blockIdx.x / pairs, pair = blockIdx.x - quad * pairs;
     const uint32_t s = pair / p.c.n_head_kv, h = pair - s * p.c.n_head_kv;
@@ -779,7 +771,7 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t i) {
 /* Equal shares of the batch's steps per wave.  A wave's first and last piece
  * may be parts of units; those of the 4 waves of a workgroup join in LDS, and
  * what is still part of a unit goes to the workspace. */
-template <class F> __global__ __launch_bounds__(256, F::OCC) void k_paged_gqa_split(const GqaParams p) {
+template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(const GqaParams p) {
     __shared__ __align__(16) float so[8][F::COLS][F::HD]; /* first and last piece of each wave */
     __shared__ float2 sml[8][F::COLS];
     __shared__ struct {
@@ -944,11 +936,12 @@ template <int HD, int T> __global__ __launch_bounds__(T < 256 ? 256 : T) void k_
 
 /* ---- host: forms, split, scratch ------------------------------------------------ */
 constexpr uint32_t kCus        = 256u;
-constexpr uint32_t kGroupSteps = 24u;
+constexpr uint32_t kWaves      = 8u * kCus; /* two per SIMD */
+constexpr uint32_t kGroupSteps = 128u;
 
 struct Launch {
     lfm_q4_plan plan;
-    uint32_t copies, tiles, occ; /* R, NT and OCC of the form */
+    uint32_t copies, tiles; /* R and NT of the form */
     enum { kDirect, kSplit, kGroup } how;
     size_t o_bytes, ml_bytes, range_bytes;
 };
@@ -967,14 +960,11 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     p.capacity  = capacity;
     L->tiles    = 1u;
     L->copies   = 1u;
-    L->occ      = 2u;
     if (head_dim == 64u) {
         if (cols <= 4u) L->copies = 4u;
         if (cols > 16u) L->tiles = 2u;
     } else {
         if (cols <= 8u) L->copies = 2u;
-        if (cols > 8u) L->occ = 1u;
-        if (cols > 16u) L->tiles = 2u;
     }
     p.cols = L->copies > 1u ? 16u / L->copies : 16u * L->tiles;
     p.step_shift = L->copies == 4u ? 6u : 5u;
@@ -984,12 +974,12 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
     if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
     const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u);
-    const uint32_t resident = 4u * kCus * L->occ; /* waves */
     /* enough units fill the card by themselves; step counts of a split are 32 bits */
-    L->how = units < 2u * resident && units * (capacity / 32u) < 0x80000000ull ? Launch::kSplit : Launch::kDirect;
-    if (units <= kCus && steps <= kGroupSteps && L->occ == 2u) L->how = Launch::kGroup;
+    L->how = units < 2u * kWaves && units * (capacity / 32u) < 0x80000000ull ? Launch::kSplit : Launch::kDirect;
+    const uint64_t wait = L->copies > 1u ? 6144u : 16384u;
+    if (units <= kCus && steps <= kGroupSteps && steps * (kCus - units) <= wait) L->how = Launch::kGroup;
     uint64_t waves = units * steps;
-    if (waves > resident) waves = resident;
+    if (waves > kWaves) waves = kWaves;
     p.n_waves    = (uint32_t)((waves + 3u) / 4u * 4u);
     const uint64_t slots = L->how == Launch::kSplit ? p.n_waves / 4u + units : 0u;
     L->o_bytes     = slots * p.cols * head_dim * 4u;
@@ -1004,11 +994,9 @@ template <class F> void launch_form(const GqaParams &p, const Launch &L, hipStre
         hipLaunchKernelGGL(k_paged_gqa<F>, dim3(pairs * ((p.plan.n_ct + 3u) / 4u)), dim3(256), 0, stream, p);
         return;
     }
-    if constexpr (F::OCC > 1) {
-        if (L.how == Launch::kGroup) {
-            hipLaunchKernelGGL((k_paged_gqa_wg<F, 8>), dim3(units), dim3(512), 0, stream, p);
-            return;
-        }
+    if (L.how == Launch::kGroup) {
+        hipLaunchKernelGGL((k_paged_gqa_wg<F, 8>), dim3(units), dim3(512), 0, stream, p);
+        return;
     }
     hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
     /* a unit's pieces: a wave takes 256 / HD at a time, a workgroup of 8 waves 8 times that */
@@ -1050,18 +1038,16 @@ int launch_paged_q4_gqa(const PagedQ4 &c, const float *q, const float *gate, int
     p.range         = reinterpret_cast<uint2 *>(w + L.o_bytes + L.ml_bytes);
     if (c.head_dim == 64u) {
         if (L.copies == 4u)
-            launch_form<Form<64, 1, 4, 2, 2, 1>>(p, L, stream);
+            launch_form<Form<64, 1, 4, 2>>(p, L, stream);
         else if (L.tiles == 1u)
-            launch_form<Form<64, 1, 1, 1, 2, 2>>(p, L, stream);
+            launch_form<Form<64, 1, 1, 1>>(p, L, stream);
         else
-            launch_form<Form<64, 2, 1, 1, 2, 1>>(p, L, stream);
+            launch_form<Form<64, 2, 1, 1>>(p, L, stream);
     } else {
         if (L.copies == 2u)
-            launch_form<Form<128, 1, 2, 1, 2, 1>>(p, L, stream);
-        else if (L.tiles == 1u)
-            launch_form<Form<128, 1, 1, 1, 1, 1>>(p, L, stream);
+            launch_form<Form<128, 1, 2, 1>>(p, L, stream);
         else
-            launch_form<Form<128, 2, 1, 1, 1, 1>>(p, L, stream);
+            launch_form<Form<128, 1, 1, 1>>(p, L, stream);
     }
     return hip_status(hipGetLastError());
 }
