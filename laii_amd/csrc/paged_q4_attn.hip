@@ -355,6 +355,12 @@ __device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
                                                                   __builtin_bit_cast(ushort2v, b)));
 }
 
+/* Two fp16 magnitudes in order, as 2 bits + 0x800: wraps for those that are not finite, which come before 0. */
+__device__ __forceinline__ uint32_t finite_rank(uint32_t w) {
+    const ushort2v a = __builtin_bit_cast(ushort2v, w);
+    return __builtin_bit_cast(uint32_t, (ushort2v)(a * (ushort2v){2, 2} + (ushort2v){0x800, 0x800}));
+}
+
 /* Scores of a step before the factor cs: sum over groups of scale * (codes . q). */
 template <class F>
 __device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<F> &st, const Half<F> &k,
@@ -399,14 +405,21 @@ __device__ __forceinline__ void scores(float (&x)[F::NT][4 * F::J], const State<
     }
 }
 
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { /* halves of two fp16 */
+    return ((w & 0x7C00u) == 0x7C00u ? 0x0000FFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+}
+
 /* A step that some row does not attend whole, or with a block that has no
  * page: masked scores become -inf, V scales that no column of the lane needs
- * 0 (weights of masked keys are then 0 whatever was stored). */
+ * 0 (weights of masked keys are then 0 whatever was stored).  A scale that is not
+ * finite, of a key that one of the lane's columns attends and another does not,
+ * is taken out too; the columns that attend it get their NaN here. */
 template <class F>
-__device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &v, const State<F> &st,
-                                          bool there_a, bool there_b, uint32_t key0, uint32_t lane) {
+__device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &v, State<F> &st, bool there_a,
+                                          bool there_b, uint32_t key0, uint32_t lane) {
     constexpr int NT = F::NT, G = F::G, J = F::J;
     const uint32_t kg = lane >> 4, u = (lane & 15u) / (16u / F::R);
+    uint32_t bad = 0u;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const uint32_t t = J > 1 ? (uint32_t)j : u;
@@ -425,11 +438,43 @@ __device__ __forceinline__ void mask_step(float (&x)[F::NT][4 * F::J], Half<F> &
             if (any) keep[i / 2] |= i & 1 ? 0xFFFF0000u : 0x0000FFFFu;
         }
 #pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = g * F::SW + (J > 1 ? (j & 1) * 2 : 0) + i;
+                v.s[J > 1 ? j / 2 : 0][at / 4][at % 4] &= keep[i];
+                if (NT > 1) bad |= not_finite(v.s[J > 1 ? j / 2 : 0][at / 4][at % 4]);
+            }
+    }
+    if (NT > 1 && __any(bad != 0u)) {
+#pragma unroll
         for (int g = 0; g < G; ++g) {
-            const int w = J > 1 ? (j & 1) * 2 : 0;
-            const int at = g * F::SW + w;
-            v.s[J > 1 ? j / 2 : 0][at / 4][at % 4] &= keep[0];
-            v.s[J > 1 ? j / 2 : 0][at / 4][at % 4 + 1] &= keep[1];
+            uint32_t hit[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) hit[n] = 0u;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = g * F::SW + (J > 1 ? (j & 1) * 2 : 0) + i;
+                    uint32_t w   = v.s[J > 1 ? j / 2 : 0][at / 4][at % 4];
+                    asm volatile("" : "+v"(w)); /* worked out here anew: the masks above are not held for this */
+                    const uint32_t m = not_finite(w);
+                    /* x is -inf exactly where the column does not attend */
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if (x[n][4 * j + 2 * i] != -__builtin_inff()) hit[n] |= m & 0xFFFFu;
+                        if (x[n][4 * j + 2 * i + 1] != -__builtin_inff()) hit[n] |= m >> 16;
+                    }
+                    v.s[J > 1 ? j / 2 : 0][at / 4][at % 4] = w & ~m;
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (kg_max(hit[n]))
+#pragma unroll
+                    for (int i = 2 * g; i < 2 * g + 2; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) st.o[n][i][k] = __builtin_nanf("");
         }
     }
 }
@@ -458,9 +503,19 @@ __device__ __forceinline__ void check_step(State<F> &st, const float (&x)[F::NT]
     }
     raise |= dv > st.vmax;
     if (__any(raise)) {
-        st.vmax = max(kg_max(dv), st.vmax);
-        /* a scale that is not finite gives NaN in its own dims alone */
-        const float z = (float)__builtin_bit_cast(_Float16, (uint16_t)min(st.vmax, 0x7BFFu));
+        if (__any(dv >= 0x7C00u)) { /* a scale that is not finite gives NaN in its own dims alone */
+            dv = 0u;
+#pragma unroll
+            for (int b = 0; b < F::SB; ++b)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < F::SW; ++i) dv = pk_max_u16(dv, finite_rank(v.scales(b, g, i)));
+            dv = max(dv & 0xFFFFu, dv >> 16);
+            dv = dv > 0x800u ? (dv - 0x800u) >> 1 : 0u;
+        }
+        st.vmax       = max(kg_max(dv), st.vmax);
+        const float z = (float)__builtin_bit_cast(_Float16, (uint16_t)st.vmax);
         const float e = (z > 0.0f ? (float)__builtin_amdgcn_frexp_expf(z) : 0.0f) - kLift;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -813,15 +868,20 @@ template <class F> __global__ __launch_bounds__(256, 2) void k_paged_gqa_split(c
         uint32_t a = t - first - h * n;
         for (; t < t1 && h < nh; ++h, a = 0u) {
             const uint32_t b = n - a < t1 - t ? n : a + (t1 - t);
+            uint32_t ln = lane;
+            /* of its own in every turn, so that what hangs on it is not held in registers across pieces: 35.9 ->
+             * 33.7 us for 16 x 8 rows at 4096 keys of head_dim 128, 33.1 -> 32.4 of 64.  Forms with registers to
+             * spare lose 1 % by it. */
+            if (F::HD == 128 || F::NT > 1) asm volatile("" : "+v"(ln));
             State<F> st;
-            run_piece<F>(st, p, s, ct, h, tile, pos0, rows, tile.step0 + a, tile.step0 + b, lane);
+            run_piece<F>(st, p, s, ct, h, tile, pos0, rows, tile.step0 + a, tile.step0 + b, ln);
             join_lanes<F>(st);
             if (a == 0u && b == n) {
-                write_out<F>(st, p, s, ct, h, rows, lane);
+                write_out<F>(st, p, s, ct, h, rows, ln);
                 if (lane == 0u) p.range[e * nh + h] = make_uint2(blockIdx.x, blockIdx.x);
             } else { /* the first piece of the share, or its last */
                 const uint32_t at = in_wg * 2u + (t == t0 ? 0u : 1u);
-                put_part<F>(st, &so[at][0][0], &sml[at][0], lane);
+                put_part<F>(st, &so[at][0][0], &sml[at][0], ln);
                 if (lane == 0u) {
                     meta[at].unit = e * nh + h;
                     meta[at].s = s, meta[at].ct = ct, meta[at].h = h, meta[at].rows = rows;

@@ -353,6 +353,31 @@ def test_not_finite_keys_stay_in_their_sequence(gpu, n_rows):
     assert np.all(np.isnan(got[0, :, :4])) and np.all(np.isfinite(got[0, :, 4:])) and np.all(np.isfinite(got[1]))
 
 
+@pytest.mark.parametrize("bits", [0x7E00, 0x7C00, 0xFC00])
+@pytest.mark.parametrize("hd,nq,n_rows,window,at", [
+    (64, 4, 1, 0, 90), (64, 8, 5, 0, 92), (64, 8, 40, 0, 101), (64, 8, 40, 30, 101), (64, 8, 40, 0, 127),
+    (64, 8, 9, 7, 91), (128, 8, 1, 0, 90), (128, 16, 40, 0, 101), (128, 16, 40, 20, 96)])
+def test_not_finite_values_stay_in_the_rows_that_attend_them(gpu, hd, nq, n_rows, window, at, bits):
+    """A V scale that is not finite: NaN in its group of dims, in the rows that attend its position and nowhere else."""
+    rng = np.random.default_rng(23)
+    p, nkv = 90, 2
+    L = filled(gpu, rng, [p + n_rows], 32, nkv, hd)
+    k, v, there = L.c.rows(0, p + n_rows)
+    _, _, _, vs, _, _ = ref.place(hd)
+    where = vs[at % 32, 32]
+    L.c.pages[L.c.table[0, at // 32], 0, 0, where:where + 2] = [bits & 255, bits >> 8]
+    L.pages.upload(L.c.pages)
+    q = rng.standard_normal((1, n_rows, nq, hd)).astype(np.float32)
+    got = L.attend(q, [p], None, window)[0]
+    t = p + np.arange(n_rows)
+    hit = np.zeros((n_rows, nq, hd), bool)
+    hit[(t >= at) & ((t < at + window) | (window == 0)), :nq // nkv, 32:64] = True
+    assert np.array_equal(np.isnan(got), hit)
+    want, mag, low, big = ref.attend(q[0], k, v, there, p, window, float(1.0 / np.sqrt(np.float32(hd))))
+    off = np.abs(got - want) / ref.bound(mag, low, big, p + n_rows, hd)
+    assert np.all(off[~hit] <= 1.0), float(off[~hit].max())
+
+
 @pytest.mark.parametrize("n_rows", [1, 5, 40])
 @pytest.mark.parametrize("vscale,qscale", [(1e-3, 1.0), (1e4, 1.0), (1.0, 1e-6), (1.0, 60.0), (1e-2, 1e4)])
 def test_magnitudes(gpu, n_rows, vscale, qscale):
