@@ -56,7 +56,7 @@ LFM_IDX_FN uint32_t lfm_q4_scale(uint32_t head_dim, uint32_t v, uint32_t t, uint
  * row major, cut into tiles of `cols`.  A unit is (sequence, tile, KV head),
  * numbered in that order; its work is the steps of 2^step_shift keys that cover
  * the keys its rows attend.  The batch's N < 2^32 steps, in unit order, go to G
- * waves in equal shares (the first N % G one longer), cut at units.  The pieces
+ * waves in shares equal to within one step, cut at units.  The pieces
  * of a workgroup's waves join in LDS; what workgroup g then holds of unit v, if
  * not all of it, has partial slot g + v: along the walk g or v grows, so slots
  * are unique and below workgroups + units.  Everything here is 32-bit: a 64-bit division costs a wave more than
@@ -113,11 +113,13 @@ LFM_IDX_FN uint32_t lfm_q4_waves(const lfm_q4_plan *p, uint32_t n_steps) {
     return n_steps < p->n_waves ? n_steps : p->n_waves;
 }
 
-/* Steps [*t0, *t1) of wave g < G. */
+/* Steps [*t0, *t1) of wave g < G <= 2048: from floor(g N / G), so that a batch of
+ * equal units is cut at every unit when G is a multiple of their number (a wave
+ * with the end of one and the start of the next has two beginnings to wait for). */
 LFM_IDX_FN void lfm_q4_share(uint32_t g, uint32_t n_steps, uint32_t G, uint32_t *t0, uint32_t *t1) {
     const uint32_t q = n_steps / G, r = n_steps - q * G;
-    *t0 = g * q + (g < r ? g : r);
-    *t1 = *t0 + q + (g < r ? 1u : 0u);
+    *t0 = g * q + g * r / G;
+    *t1 = (g + 1u) * q + (g + 1u) * r / G;
 }
 
 #endif

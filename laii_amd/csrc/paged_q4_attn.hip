@@ -782,9 +782,9 @@ template <class F, int W> __global__ __launch_bounds__(64 * W, 2) void k_paged_g
     const uint32_t pos0 = scalar_at(p.c.pos0, s), rows = rows_at(p.c, s, pos0);
     const lfm_q4_tile t = lfm_q4_tile_of(&p.plan, pos0, rows, ct);
     if (t.n_steps == 0u) return;
-    uint32_t a, b;
-    lfm_q4_share(wave, t.n_steps, W, &a, &b);
-    const uint32_t parts = t.n_steps < W ? t.n_steps : W; /* the first shares are the longer ones */
+    /* the first shares are the longer ones */
+    const uint32_t more = t.n_steps % W, parts = t.n_steps < W ? t.n_steps : W;
+    uint32_t a = wave * (t.n_steps / W) + (wave < more ? wave : more), b = a + t.n_steps / W + (wave < more ? 1u : 0u);
     a = uniform(a), b = uniform(b);
     if (a < b) {
         State<F> st;
@@ -1034,13 +1034,25 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
     if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
     const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u);
-    /* enough units fill the card by themselves; step counts of a split are 32 bits */
-    L->how = units < 2u * kWaves && units * (capacity / 32u) < 0x80000000ull ? Launch::kSplit : Launch::kDirect;
-    const uint64_t wait = L->copies > 1u ? 6144u : 16384u;
+    /* Enough units fill the card by themselves, a wave each; unless they are whole sequences with long contexts,
+     * which end one after the other at their own lengths.  Us, wave per unit | split, 800 x 1 rows of head_dim 64:
+     * 100 keys each 36.6 | 48.7, up to 600 keys 65.9 | 77.7, 2000 keys each 232 | 195, up to 2000 keys 157 | 134.
+     * Step counts of a split are 32 bits. */
+    L->how = (units < 2u * kWaves || (p.n_ct == 1u && keys >= 1024u)) && units * (capacity / 32u) < 0x80000000ull
+                 ? Launch::kSplit : Launch::kDirect;
+    /* A workgroup per unit has no second launch and no partials, 2 to 8 us (the more units, the more), but only
+     * `units` of the 256 CUs work: it is ahead while steps * (256 - units) is small.  Us, group | split, at
+     * 16 x 8 rows of head_dim 64 (128 units): 2000 keys 19.8 | 21.1, 4000 keys 31.1 | 26.8; 4 rows (16 columns,
+     * half the work a step): 2000 keys 13.8 | 15.1, 4000 keys 21.2 | 19.0; 1 row of 8 sequences: 2000 keys
+     * 12.2 | 12.6, 4000 keys 17.4 | 14.6.  Up to 128 steps, so that a long sequence among short ones is split. */
+    const uint64_t wait = head_dim == 128u || L->copies > 1u ? 7168u : L->tiles > 1u ? 9216u : 12288u;
     if (units <= kCus && steps <= kGroupSteps && steps * (kCus - units) <= wait) L->how = Launch::kGroup;
     uint64_t waves = units * steps;
     if (waves > kWaves) waves = kWaves;
-    p.n_waves    = (uint32_t)((waves + 3u) / 4u * 4u);
+    p.n_waves = (uint32_t)((waves + 3u) / 4u * 4u);
+    /* whole workgroups per unit, where that leaves few waves out */
+    const uint32_t even = (uint32_t)(p.n_waves / (4u * units) * (4u * units));
+    if (even >= p.n_waves - p.n_waves / 16u) p.n_waves = even;
     const uint64_t slots = L->how == Launch::kSplit ? p.n_waves / 4u + units : 0u;
     L->o_bytes     = slots * p.cols * head_dim * 4u;
     L->ml_bytes    = slots * p.cols * 8u;

@@ -37,6 +37,8 @@ typedef struct {
         goto out;                                                                                                     \
     } while (0)
 
+void share(uint32_t g, uint32_t n_steps, uint32_t G, uint32_t *t0, uint32_t *t1) { lfm_q4_share(g, n_steps, G, t0, t1); }
+
 int plan_check(uint32_t n_seq, const uint32_t *pos0, const uint32_t *rows_seq, uint32_t n_rows, uint32_t kv_mul,
                uint32_t n_head_kv, uint32_t window, uint32_t capacity, uint32_t cols, uint32_t step_shift,
                uint32_t n_waves, int mutant, char *msg, size_t msg_len) {

@@ -486,3 +486,17 @@ def test_pages_past_4_gib(gpu):
     assert np.array_equal(gk[0], c.rows(0, n)[0].astype(np.float32).astype(np.float16))
     q = rng.standard_normal((1, 1, 32, hd)).astype(np.float32)
     check_attend(L, L.attend(q, [n - 1]), q, [n - 1])
+
+
+def test_many_sequences_and_a_long_one(gpu):
+    """More sequences than the card has waves for, lengths from none to thousands of keys."""
+    rng = np.random.default_rng(24)
+    n = 1030
+    pos = rng.integers(0, 40, n)
+    pos[[0, 511, 1029]] = [3000, 700, 2047]
+    rows = np.ones(n, int)
+    rows[rng.integers(1, n - 1, 200)] = 0
+    L = filled(gpu, rng, [int(p) + 1 for p in pos], 32, 4, 64)
+    q = rng.standard_normal((n, 1, 8, 64)).astype(np.float32)
+    for hint in (None, 100):
+        check_attend(L, L.attend(q, pos, rows, hint=hint), q, pos, rows)

@@ -30,6 +30,8 @@ def sim(tmp_path_factory):
                             n_rows, mul, nkv, window, capacity, cols, shift, waves, mutant, msg, 256)
         return rc, msg.value.decode()
 
+    check.lib = lib
+    lib.share.argtypes = [C.c_uint32] * 3 + [U32P] * 2
     return check
 
 
@@ -59,6 +61,19 @@ def test_ends(sim, pos, rows, n_rows):
         for waves in (4, 2048):
             rc, msg = sim(pos, n_rows, 4, 1, window, 2 ** 31, 16, 5, waves, rows)
             assert rc == 0, (window, waves, rc, msg)
+
+
+@pytest.mark.parametrize("units,n_steps,k", [(128, 129, 4), (8, 2049, 256), (24, 77, 84), (3, 1000, 680), (512, 9, 4)])
+def test_equal_units_are_cut_at_their_ends(sim, units, n_steps, k):
+    """k waves for each of equal units: none holds the end of one and the start of the next."""
+    waves, k = -(-units * k // 4) * 4, min(k, n_steps)  # a wave has a step at least
+    for u in range(units):
+        for g in (u * k, u * k + k - 1):
+            t0, t1 = C.c_uint32(), C.c_uint32()
+            sim.lib.share(g, units * n_steps, units * k, C.byref(t0), C.byref(t1))
+            assert u * n_steps <= t0.value < t1.value <= (u + 1) * n_steps
+            assert g != u * k or t0.value == u * n_steps
+    assert sim([n_steps * 32 - 1] * units, 1, 4, 1, 0, 1 << 20, 16, 5, waves)[0] == 0
 
 
 @pytest.mark.parametrize("mutant", [1, 2, 3])
