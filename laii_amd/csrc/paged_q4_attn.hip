@@ -1071,8 +1071,10 @@ template <class F> void launch_form(const GqaParams &p, const Launch &L, hipStre
         return;
     }
     hipLaunchKernelGGL(k_paged_gqa_split<F>, dim3(p.plan.n_waves / 4u), dim3(256), 0, stream, p);
-    /* a unit's pieces: a wave takes 256 / HD at a time, a workgroup of 8 waves 8 times that */
-    if (p.plan.n_waves / 4u <= 16u * units)
+    /* A unit's pieces: a wave takes 256 / HD at a time, a workgroup 8 times that.  Up to 4 turns of a wave; us, wave |
+     * workgroup: head_dim 64, 16 pieces, 4 x 8 rows: 16.1 | 19.3; head_dim 128, 16 pieces, 8 x 1 rows of 5000 keys:
+     * 19.0 | 17.4. */
+    if (p.plan.n_waves / 4u * F::HD <= 1024u * units)
         hipLaunchKernelGGL((k_paged_merge<F::HD, 64>), dim3((cols + 3u) / 4u), dim3(256), 0, stream, p);
     else
         hipLaunchKernelGGL((k_paged_merge<F::HD, 512>), dim3(cols), dim3(512), 0, stream, p);
