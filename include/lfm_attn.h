@@ -521,7 +521,9 @@ int lfm_hip_paged_q4_gather(uint16_t *k_out, uint16_t *v_out, const void *pages,
  * pos_0[s] + r, t_start(p) = p + 1 - window_len where window_len > 0 and
  * p + 1 > window_len, else 0.  gate as in lfm_hip_gqa_f16_varlen.  A row that
  * finds no page at all gives zeros.  Outputs have fp32 accuracy with respect to
- * the cached values.
+ * the cached values: a few 2^-20 of sum p |v|, and below that 2^-30 of the head's
+ * largest |v| for every attended key, relative to the largest weight.  A cached
+ * value that is not finite reaches only rows that attend its position.
  * q, out: [n_seq][n_rows][n_head_q][head_dim], n_head_q a multiple of n_head_kv;
  * q rotated.
  * keys_hint: an upper bound of pos_0[s] + rows over the batch (0 = what the

