@@ -230,8 +230,8 @@ int lfm_hip_quantize_q8_K(const float *x, void *y_q8_K, uint32_t n_rows, uint32_
  *       stored).
  * The mean and y are formed in 64 bits and rounded once.  y and y_q8_K share
  * no memory with the other arrays.  n_cols % 256 == 0 (else
- * LFM_ATTN_E_UNSUPPORTED), at most 2^24; n_rows < 2^31; n_rows == 0 does
- * nothing.  Float arrays 16-byte aligned, y_q8_K 4-byte. */
+ * LFM_ATTN_E_UNSUPPORTED), at most 2^24; n_rows < 2^24 (else the same);
+ * n_rows == 0 does nothing.  Float arrays 16-byte aligned, y_q8_K 4-byte. */
 int lfm_hip_add_rmsnorm_q8_K(const float *x, const float *residual, const float *norm_w, float eps,
                              float *residual_out, float *y, void *y_q8_K, uint32_t n_rows, uint32_t n_cols,
                              lfm_attn_stream_t stream);
@@ -480,8 +480,9 @@ int lfm_hip_lfm3_prefill_f16(const float *q, const uint16_t *k, const uint16_t *
  * Rows behind a sequence's last, and rows at positions that the table
  * (table_stride * page_size positions, at most 2^31) does not reach, are left as
  * they were in every output.  Positions without a page are not stored, not
- * attended, and read back as zeros.  head_dim 64 or 128, page_size as above, else
- * LFM_ATTN_E_UNSUPPORTED.  Row arrays, tables of cosines and norm weights
+ * attended, and read back as zeros.  head_dim 64 or 128, page_size as above, and
+ * a batch of less than 2^24 workgroups (of 32 positions of a KV head, or 64 or
+ * 128 query columns), else LFM_ATTN_E_UNSUPPORTED.  Row arrays, tables of cosines and norm weights
  * 16-byte aligned. */
 /* Bytes of one page. */
 int lfm_attn_paged_q4_page_bytes(uint32_t page_size, uint32_t n_head_kv, uint32_t head_dim, size_t *bytes);
@@ -497,8 +498,9 @@ int lfm_attn_paged_q4_page_bytes(uint32_t page_size, uint32_t n_head_kv, uint32_
  * q, q_out: [n_seq][n_rows][n_head_q][head_dim]; k, v:
  * [n_seq][n_rows][n_head_kv][head_dim].  cos_lut / sin_lut:
  * [lut_rows][head_dim / 2]; rows at positions >= lut_rows count as rows behind
- * the last.  Two sequences of a call must not store into the same block of 32
- * positions of a page (shared pages are for prefixes that are only read). */
+ * the last.  No two table entries of a call may lead stored rows into the same
+ * block of 32 positions of a page (shared pages are for prefixes that are only
+ * read). */
 int lfm_hip_paged_q4_append(const float *q, const float *k, const float *v, float *q_out, void *pages,
                             uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
                             uint32_t table_stride, const uint32_t *pos_0, const uint32_t *n_rows_seq,
@@ -525,7 +527,7 @@ int lfm_hip_paged_q4_gather(uint16_t *k_out, uint16_t *v_out, const void *pages,
  * largest |v| for every attended key, relative to the largest weight.  A cached
  * value that is not finite reaches only rows that attend its position.
  * q, out: [n_seq][n_rows][n_head_q][head_dim], n_head_q a multiple of n_head_kv;
- * q rotated.
+ * q rotated.  scale: finite, any sign.
  * keys_hint: an upper bound of pos_0[s] + rows over the batch (0 = what the
  * table reaches); it sizes the key split.  Longer sequences are still handled
  * correctly, with longer shares.

@@ -270,10 +270,13 @@ uint32_t blocks_met(uint32_t n_rows) { return (n_rows + 30u) / 32u + 1u; }
 } // namespace
 
 bool paged_q4_append_fits(const PagedQ4 &c, uint32_t n_head_q) {
-    const uint64_t heads = 256u / (c.head_dim / 8u);
-    const uint64_t kv    = (uint64_t)c.n_seq * blocks_met(c.n_rows) * c.n_head_kv;
-    const uint64_t q     = ((uint64_t)c.n_seq * c.n_rows * n_head_q + heads - 1u) / heads;
-    return kv + q <= 0x7FFFFFFFull;
+    /* of 256 threads each: a launch's threads are 32 bits */
+    const uint64_t limit = 1ull << 24, heads = 256u / (c.head_dim / 8u);
+    uint64_t kv, q;
+    if (__builtin_mul_overflow((uint64_t)c.n_seq * blocks_met(c.n_rows), (uint64_t)c.n_head_kv, &kv) ||
+        __builtin_mul_overflow((uint64_t)c.n_seq * c.n_rows, (uint64_t)n_head_q, &q))
+        return false;
+    return kv < limit && q < limit * heads && kv + (q + heads - 1u) / heads < limit;
 }
 
 int launch_paged_q4_append(const PagedQ4 &c, const float *q, const float *k, const float *v, float *q_out,

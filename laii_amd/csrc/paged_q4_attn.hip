@@ -328,7 +328,8 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
                 big = fmaxf(big, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
             }
         big = kg_max(big);
-        const int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
+        int e = big > 0.0f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) : 0;
+        if (e < -100) e = -100; /* 2^-e stays finite; such scores are 0 in fp32 */
         const float unit = ldexpf(p.scale < 0.0f ? -1.0f : 1.0f, -e);
 #pragma unroll
         for (int g = 0; g < F::G; ++g) {
@@ -352,8 +353,10 @@ __device__ __forceinline__ void start(State<F> &st, const GqaParams &p, uint32_t
             }
             st.c0[n][g] = ldexpf(-8.0f * kg_sum(sum), -kKDown);
         }
-        /* never 0: a masked score is cs * -inf */
-        st.cs[n]  = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e + kKDown), 1e-37f);
+        /* Never 0: a masked score is cs * -inf.  At most 2^80: scores stay below 2^96, far from kNoScore, and where
+         * that cuts, different scores (by 2^-68 before the factor, or more) are still 2^12 apart, so one weight is 1
+         * and the others 0 as they should be. */
+        st.cs[n]  = fminf(fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, e + kKDown), 1e-37f), 0x1p80f);
         st.top[n] = st.m[n] = kNoScore;
         st.l[n] = 0.0f;
         st.vmax = 0u;
@@ -1042,8 +1045,10 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     p.cols = L->copies > 1u ? 16u / L->copies : 16u * L->tiles;
     p.step_shift = L->copies == 4u ? 6u : 5u;
     p.n_ct = (uint32_t)((cols + p.cols - 1u) / p.cols);
-    const uint64_t entries = (uint64_t)n_seq * p.n_ct, units = entries * n_head_kv;
-    if (units > 0x7FFFFFFFull / p.cols) return LFM_ATTN_E_UNSUPPORTED;
+    /* the threads of a launch are 32 bits: 256 per 4 tiles, and 64 per column in a merge (below) */
+    const uint64_t pairs = (uint64_t)n_seq * n_head_kv;
+    if (pairs >= 1ull << 24 || pairs * ((p.n_ct + 3u) / 4u) >= 1ull << 24) return LFM_ATTN_E_UNSUPPORTED;
+    const uint64_t units = pairs * p.n_ct;
     uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
     if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
     const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u);
@@ -1051,8 +1056,8 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
      * which end one after the other at their own lengths.  Us, wave per unit | split, 800 x 1 rows of head_dim 64:
      * 100 keys each 36.6 | 48.7, up to 600 keys 65.9 | 77.7, 2000 keys each 232 | 195, up to 2000 keys 157 | 134.
      * Step counts of a split are 32 bits. */
-    L->how = (units < 2u * kWaves || (p.n_ct == 1u && keys >= 1024u)) && units * (capacity / 32u) < 0x80000000ull
-                 ? Launch::kSplit : Launch::kDirect;
+    const bool fits = units * (capacity / 32u) < 1ull << 31 && units * p.cols < 1ull << 26;
+    L->how = fits && (units < 2u * kWaves || (p.n_ct == 1u && keys >= 1024u)) ? Launch::kSplit : Launch::kDirect;
     /* A workgroup per unit has no second launch and no partials, 2 to 8 us (the more units, the more), but only
      * `units` of the 256 CUs work: it is ahead while steps * (256 - units) is small.  Us, group | split, at
      * 16 x 8 rows of head_dim 64 (128 units): 2000 keys 19.8 | 21.1, 4000 keys 31.1 | 26.8; 4 rows (16 columns,

@@ -371,7 +371,7 @@ int lfm_hip_add_rmsnorm_q8_K(const float *x, const float *residual, const float 
                              lfm_attn_stream_t stream) {
     if (n_rows == 0u) return LFM_ATTN_OK;
     if (!x || (!residual_out && !y && !y_q8_K) || n_cols == 0u || n_rows >= 0x80000000u) return LFM_ATTN_E_INVALID;
-    if (n_cols % 256u || n_cols > (1u << 24)) return LFM_ATTN_E_UNSUPPORTED;
+    if (n_cols % 256u || n_cols > (1u << 24) || n_rows >= (1u << 24)) return LFM_ATTN_E_UNSUPPORTED;
     if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(norm_w, 16) || !aligned(residual_out, 16) ||
         !aligned(y, 16) || !aligned(y_q8_K, 4))
         return LFM_ATTN_E_INVALID;
@@ -714,7 +714,7 @@ static int paged_cache(lfm::PagedQ4 *c, const void *pages, uint32_t n_pages, uin
     if (!aligned(pages, 16) || !aligned(block_table, 4) || !aligned(pos_0, 4) || !aligned(n_rows_seq, 4))
         return LFM_ATTN_E_INVALID;
     const uint64_t reach = (uint64_t)table_stride * page_size;
-    if (reach > 0x80000000ull || n_pages > 0x7FFFFFFFu) return LFM_ATTN_E_UNSUPPORTED;
+    if (reach > 0x80000000ull || n_pages > 0x7FFFFFFFu || n_rows > 0x7FFFFFFFu) return LFM_ATTN_E_UNSUPPORTED;
     c->pages        = static_cast<uint8_t *>(const_cast<void *>(pages));
     c->table        = block_table;
     c->pos0         = pos_0;
@@ -797,7 +797,7 @@ int lfm_hip_paged_q4_gqa(const float *q, const float *gate, int gate_is_logit, c
                          n_head_kv, head_dim);
     if (st != LFM_ATTN_OK) return st;
     if (!q || !out || n_head_q == 0u || n_head_q % n_head_kv != 0u || !aligned(q, 16) || !aligned(out, 16) ||
-        !aligned(gate, 4) || !aligned(workspace, 16))
+        !aligned(gate, 4) || !aligned(workspace, 16) || !__builtin_isfinite(scale))
         return LFM_ATTN_E_INVALID;
     size_t need = 0;
     st = lfm::paged_q4_gqa_workspace(n_seq, n_rows, keys_hint, n_head_q, n_head_kv, head_dim, c.capacity, window_len,

@@ -500,3 +500,55 @@ def test_many_sequences_and_a_long_one(gpu):
     q = rng.standard_normal((n, 1, 8, 64)).astype(np.float32)
     for hint in (None, 100):
         check_attend(L, L.attend(q, pos, rows, hint=hint), q, pos, rows)
+
+
+@pytest.mark.parametrize("n_rows", [1, 5, 40])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-20, 2.0])
+def test_scales(gpu, n_rows, scale):
+    rng = np.random.default_rng(25)
+    pos = [130, 7]
+    L = filled(gpu, rng, [p + n_rows for p in pos], 32, 2, 64)
+    q = rng.standard_normal((2, n_rows, 8, 64)).astype(np.float32)
+    check_attend(L, L.attend(q, pos, scale=scale), q, pos, scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("n_rows", [1, 5, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_smallest_and_largest_queries(gpu, hd, n_rows):
+    """Queries below the normal numbers: all weights alike.  Queries whose scores come near fp32's end or pass it: one
+    weight is 1, the others 0, as long as the best score leads by far more than the scores' rounding, so what
+    remains is the error of p d as hi + lo, 2^-20 of |v|."""
+    rng = np.random.default_rng(26)
+    pos = 70
+    L = filled(gpu, rng, [pos + n_rows], 32, 2, hd)
+    unit = rng.standard_normal((1, n_rows, 8, hd)).astype(np.float32)
+    for size in (1e-45, 1e-41, 1e-38, 1e-30):
+        q = (size * unit).astype(np.float32)
+        check_attend(L, L.attend(q, [pos]), q, [pos])
+    k, v, _ = L.c.rows(0, pos + n_rows)
+    for size in (1e20, 1e32, 5e37):
+        q = (size * unit).astype(np.float32)
+        got = L.attend(q, [pos])[0]
+        for r in range(n_rows):
+            for h in range(8):
+                s = k[:pos + r + 1, h // 4] @ q[0, r, h].astype(np.float64)
+                first, second = np.argsort(s)[:-3:-1]
+                if s[first] - s[second] < 2.0 ** -12 * np.abs(s).max():
+                    continue
+                want = v[first, h // 4]
+                assert np.all(np.abs(got[r, h] - want) <= 2.0 ** -20 * np.abs(want)), (size, r, h)
+
+
+@pytest.mark.parametrize("n_rows", [1, 5, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_not_finite_queries_stay_in_their_head(gpu, hd, n_rows):
+    rng = np.random.default_rng(27)
+    pos = [90, 40]
+    L = filled(gpu, rng, [p + n_rows for p in pos], 32, 2, hd)
+    q = rng.standard_normal((2, n_rows, 8, hd)).astype(np.float32)
+    good = L.attend(q, pos)
+    q[0, 0, 1, 5], q[1, n_rows - 1, 7, 40] = np.nan, np.inf
+    got = L.attend(q, pos)
+    bad = np.zeros(got.shape, bool)
+    bad[0, 0, 1] = bad[1, n_rows - 1, 7] = True
+    assert np.all(np.isnan(got[bad])) and np.array_equal(got[~bad], good[~bad])

@@ -45,7 +45,7 @@ def norm_args(**kw):
 @pytest.mark.parametrize("change,status", [
     (dict(n=0), OK), (dict(n=0, cols=3), OK), (dict(x=None), E_INVALID), (dict(out=None, y=None, q=None), E_INVALID),
     (dict(cols=0), E_INVALID), (dict(cols=255), E_UNSUPPORTED), (dict(cols=(1 << 24) + 256), E_UNSUPPORTED),
-    (dict(n=1 << 31), E_INVALID), (dict(x=ODD), E_INVALID), (dict(res=ODD), E_INVALID), (dict(w=ODD), E_INVALID),
+    (dict(n=1 << 31), E_INVALID), (dict(n=1 << 24), E_UNSUPPORTED), (dict(x=ODD), E_INVALID), (dict(res=ODD), E_INVALID), (dict(w=ODD), E_INVALID),
     (dict(out=ODD), E_INVALID), (dict(y=ODD), E_INVALID), (dict(q=FAKE + 2), E_INVALID)])
 def test_norm_refusals(change, status):
     assert la.load().lfm_hip_add_rmsnorm_q8_K(*norm_args(**change)) == status
@@ -130,3 +130,24 @@ def test_attention_refuses_a_small_workspace(n_seq, n_rows, hint, hd, nq, nkv):
             la.paged_q4_gqa(FAKE, None, True, FAKE, 10, 64, FAKE, 200, FAKE, None, FAKE, n_seq, n_rows, hint, nq, nkv,
                             hd, work, size)
         assert e.value.status == status, (work, size)
+
+
+HUGE = [dict(n_seq=0xFFFFFFFF, n_rows=0x7FFFFFFF, nkv=4096), dict(n_rows=0xFFFFFFFF), dict(n_rows=0x80000000),
+        dict(n_seq=0xFFFFFFFF, nkv=4096), dict(n_seq=1 << 23, nkv=2), dict(n_seq=1, nkv=1, n_rows=0xFFFFFFE4)]
+
+
+@pytest.mark.parametrize("change", HUGE)
+def test_sizes_whose_products_pass_a_launch(change):
+    """Refused, in whatever way the products would wrap."""
+    assert append(**change, nq=4096) == E_UNSUPPORTED
+    assert gather(**change) == E_UNSUPPORTED
+    assert gqa(**change, nq=4096) == E_UNSUPPORTED
+    with pytest.raises(la.LfmAttnError) as e:
+        la.paged_q4_workspace_bytes(change.get("n_seq", 2), change.get("n_rows", 1), 0, 4096, change.get("nkv", 2), 64,
+                                    64, 4)
+    assert e.value.status == E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_scales_that_are_not_finite(scale):
+    assert gqa(scale=scale) == E_INVALID
