@@ -1050,14 +1050,23 @@ int plan_launch(Launch *L, uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, 
     if (pairs >= 1ull << 24 || pairs * ((p.n_ct + 3u) / 4u) >= 1ull << 24) return LFM_ATTN_E_UNSUPPORTED;
     const uint64_t units = pairs * p.n_ct;
     uint64_t keys = keys_hint && keys_hint < capacity ? keys_hint : capacity;
-    if (window && window + (uint64_t)n_rows < keys) keys = window + (uint64_t)n_rows;
-    const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u);
-    /* Enough units fill the card by themselves, a wave each; unless they are whole sequences with long contexts,
-     * which end one after the other at their own lengths.  Us, wave per unit | split, 800 x 1 rows of head_dim 64:
-     * 100 keys each 36.6 | 48.7, up to 600 keys 65.9 | 77.7, 2000 keys each 232 | 195, up to 2000 keys 157 | 134.
-     * Step counts of a split are 32 bits. */
-    const bool fits = units * (capacity / 32u) < 1ull << 31 && units * p.cols < 1ull << 26;
-    L->how = fits && (units < 2u * kWaves || (p.n_ct == 1u && keys >= 1024u)) ? Launch::kSplit : Launch::kDirect;
+    const uint64_t span = p.n_ct > 1u ? p.cols / mul + 2u : n_rows; /* rows that a tile may meet */
+    if (window && window + span < keys) keys = window + span;
+    const uint64_t steps = (keys >> p.step_shift) + 1u + (window ? 1u : 0u); /* of the longest unit */
+    /* A wave per unit, or equal shares of all steps (whose counts, and whose merge's threads, are 32 bits).  In
+     * 1 / 1450 us: a wave takes its unit's steps one after the other, 1340 each alone on a SIMD, 2060 beside a second
+     * one, and decodes that fill the card are bound by memory, which units of one length each use worse; a split
+     * takes the mean, and a start, pieces and merge by the unit.  Us, wave per unit | split: prompts, head_dim 64:
+     * 4 x 600 rows 30 | 93, 1 x 4000 rows 176 | 399, 4 x 500 rows from position 2000 112 | 140, 1 x 700 from 1000
+     * 52 | 49, 1 x 300 from 8000 222 | 75; single rows: 96 x 250 keys 8.6 | 16.7, 96 x 2000 31.1 | 32.3, 256 x 500
+     * 28.7 | 25.2, 256 x up to 500 24.4 | 31.4, 256 x 2000 83.5 | 60.8; head_dim 128: 160 x 500 19.5 | 25.9,
+     * 160 x 2000 57.3 | 49.6. */
+    const uint64_t early = (n_rows >> p.step_shift) / 2u, mean = window || steps <= early ? steps : steps - early;
+    uint64_t apart       = steps * (units > kWaves / 2u ? 2060u : 1340u);
+    if (p.n_ct == 1u && units > kWaves / 2u && 2u * units * steps > apart) apart = 2u * units * steps;
+    const uint64_t even_cost = units * mean + (L->copies > 1u ? 10u : 32u) * units + 10000u;
+    const bool can_split     = units * (capacity / 32u) < 1ull << 31 && units * p.cols < 1ull << 26;
+    L->how = can_split && apart > even_cost ? Launch::kSplit : Launch::kDirect;
     /* A workgroup per unit has no second launch and no partials, 2 to 8 us (the more units, the more), but only
      * `units` of the 256 CUs work: it is ahead while steps * (256 - units) is small.  Us, group | split, at
      * 16 x 8 rows of head_dim 64 (128 units): 2000 keys 19.8 | 21.1, 4000 keys 31.1 | 26.8; 4 rows (16 columns,
