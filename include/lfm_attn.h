@@ -534,9 +534,8 @@ int lfm_hip_paged_q4_gather(uint16_t *k_out, uint16_t *v_out, const void *pages,
  * workspace: device scratch of the caller, 16-byte aligned, of at least
  * lfm_attn_paged_q4_workspace_bytes for these arguments (else
  * LFM_ATTN_E_SCRATCH, nothing launched; a larger batch may need less).  It needs
- * no initial value and holds
- * nothing between calls; calls that may overlap need one each.  The call
- * allocates nothing and may be captured. */
+ * no initial value and holds nothing between calls; calls that may overlap need
+ * one each.  The call allocates nothing and may be captured. */
 int lfm_attn_paged_q4_workspace_bytes(uint32_t n_seq, uint32_t n_rows, uint32_t keys_hint, uint32_t n_head_q,
                                       uint32_t n_head_kv, uint32_t head_dim, uint32_t page_size,
                                       uint32_t table_stride, uint32_t window_len, size_t *bytes);

@@ -552,3 +552,30 @@ def test_not_finite_queries_stay_in_their_head(gpu, hd, n_rows):
     bad = np.zeros(got.shape, bool)
     bad[0, 0, 1] = bad[1, n_rows - 1, 7] = True
     assert np.all(np.isnan(got[bad])) and np.array_equal(got[~bad], good[~bad])
+
+
+@pytest.mark.parametrize("hint", [1, 700, 20000])
+@pytest.mark.parametrize("hd,nq,nkv,n_rows,window", [
+    (64, 8, 2, 40, 0), (64, 8, 2, 150, 0), (64, 8, 2, 150, 90), (64, 2, 2, 150, 0), (128, 8, 2, 40, 0),
+    (128, 6, 2, 150, 0), (128, 8, 2, 150, 33)])
+def test_prompt_rows_in_every_division_of_the_work(gpu, hd, nq, nkv, n_rows, window, hint):
+    """The bound of the keys chooses between a wave or workgroup per tile and equal shares; the result may not."""
+    rng = np.random.default_rng(28)
+    pos, rows = [500, 0, 61, 0], [n_rows, n_rows - 7, n_rows // 2, 0]
+    c = ref.Cache(rng, [p + r for p, r in zip(pos, rows)][:3] + [20000], 64, nkv, hd)  # a table of 20000 positions
+    for s in range(3):
+        k, v = (rng.standard_normal((pos[s] + rows[s], nkv, hd)).astype(np.float32) for _ in range(2))
+        c.store(s, 0, k, v)
+    L = Layer(gpu, c)
+    q = rng.standard_normal((4, n_rows, nq, hd)).astype(np.float32)
+    check_attend(L, L.attend(q, pos, rows, window, hint=hint), q, pos, rows, window)
+
+
+@pytest.mark.parametrize("hd,nq,n_rows", [(64, 4, 40), (128, 4, 20), (64, 1, 3)])
+def test_long_windows_in_a_split(gpu, hd, nq, n_rows):
+    rng = np.random.default_rng(29)
+    pos, window = [3000, 700], 2500
+    L = filled(gpu, rng, [p + n_rows for p in pos], 64, 1, hd)
+    assert gpu.paged_q4_workspace_bytes(2, n_rows, 3000 + n_rows, nq, 1, hd, 64, L.c.stride, window) > 0
+    q = rng.standard_normal((2, n_rows, nq, hd)).astype(np.float32)
+    check_attend(L, L.attend(q, pos, None, window), q, pos, None, window)
